@@ -88,7 +88,7 @@ void gemm_bf16(const Tensor& a, const Tensor& b, Tensor& d, bool a_mn, bool b_mn
   const int64_t K = a_mn ? a.size(0) : a.size(1);
   const int64_t N = b_mn ? b.size(1) : b.size(0);
   const int64_t Kb = b_mn ? b.size(0) : b.size(1);
-  TORCH_CHECK(K == Kb, "gemm: K mismatch ", K, " vs ", Kb);
+  TORCH_CHECK(K == Kb, "gemm: K mismatch ", std::to_string(K), " vs ", std::to_string(Kb));
   TORCH_CHECK(d.size(0) == M && d.size(1) == N, "gemm: output shape mismatch");
   if (M == 0 || N == 0) return;
   TORCH_CHECK(K > 0, "gemm: K must be positive");
