@@ -13,6 +13,7 @@
 #include <pybind11/stl.h>
 
 #include "host/kv_allocator.h"
+#include "bindings_cache.h"
 #include "bindings_layers.h"
 #include "host/packer.h"
 #include "launchers.h"
@@ -414,7 +415,7 @@ LayerArgs layer_args(const Tensor& params, const std::vector<int64_t>& offs, con
   a.T = (int)x.size(0);
   const int64_t n = params.numel(), H = a.H;
   const int64_t ends[7] = {a.ln1 + H, a.wqkv + H * a.qkv(), a.bqkv < 0 ? 0 : a.bqkv + a.qkv(), a.wo + H * a.qd(), a.ln2 + H, a.wgu + 2 * H * a.F, a.wd + H * a.F};
-  for (int i = 0; i < 7; ++i) TORCH_CHECK(ends[i] <= n && (i == 2 || offs[i] >= 0) && (offs[i] < 0 || offs[i] % 8 == 0), "layer: offset of tensor ", i);
+  for (int i = 0; i < 7; ++i) TORCH_CHECK(ends[i] <= n && (i == 2 || offs[i] >= 0) && (offs[i] < 0 || offs[i] % 8 == 0), "layer: offset of tensor ", std::to_string(i));
   TORCH_CHECK(a.H % 8 == 0 && a.F % 8 == 0 && a.qd() % 8 == 0 && (reinterpret_cast<uintptr_t>(a.params) & 15) == 0, "layer: rows of 16 bytes");
   return a;
 }
@@ -677,7 +678,22 @@ void lmhead_backward(const Tensor& hidden, const Tensor& weight, const Tensor& l
 }
 
 void kv_cache_write(const Tensor& qkv, const Tensor& slots, Tensor& k_cache, Tensor& v_cache, int64_t Hq, int64_t Hkv, int64_t D,
-                    const OptTensor& status, int64_t kv_head0) {
+                    const OptTensor& status, int64_t kv_head0, const OptTensor& k_scale, const OptTensor& v_scale) {
+  if (k_cache.scalar_type() != torch::kBFloat16) {  // 8 bits
+    const char* op = "kv_cache_write";
+    TORCH_CHECK(Hq >= 0 && Hkv > 0 && kv_head0 >= 0, op, ": heads");
+    cache_args::rows(qkv, (Hq + 2 * Hkv) * D, op, "qkv");
+    const agrpo::PagedCache c = cache_args::cache(k_cache, v_cache, k_scale, v_scale, qkv.device(), D, op);
+    TORCH_CHECK(c.Hkv + kv_head0 <= Hkv, op, ": cache [blocks, kv heads of this rank, bs, D]");
+    cache_args::ints(slots, qkv.device(), 0, op, "slots");
+    TORCH_CHECK(slots.numel() == qkv.size(0), op, ": a slot for each row");
+    cache_args::status_word(status, qkv.device(), op);
+    const c10::cuda::CUDAGuard guard(qkv.device());
+    agrpo::launch_kv8_write(qkv.data_ptr(), qkv.stride(0), (int)((Hq + kv_head0) * D), (int)((Hq + Hkv + kv_head0) * D), slots.data_ptr<int>(), c,
+                            (int)qkv.size(0), opt_ptr<int>(status), cur_stream());
+    return;
+  }
+  TORCH_CHECK(!cache_args::given(k_scale) && !cache_args::given(v_scale), "kv_cache_write: a bf16 cache has no scales");
   check_bf16(qkv, "qkv"); check_i32(slots, "slots"); check_bf16(k_cache, "k_cache"); check_bf16(v_cache, "v_cache");
   TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(0) % 8 == 0, "kv_cache_write: qkv");
   TORCH_CHECK(k_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() && k_cache.size(1) + kv_head0 <= Hkv && kv_head0 >= 0 && k_cache.size(3) == D,
@@ -705,7 +721,31 @@ void kv_cache_write_decode(const Tensor& qkv, const Tensor& block_tables, const 
 }
 
 void rope_kv_write_decode(Tensor& qkv, const Tensor& cos_t, const Tensor& sin_t, const Tensor& block_tables, const Tensor& seq_lens,
-                          Tensor& k_cache, Tensor& v_cache, int64_t Hq, int64_t Hkv, int64_t D, const OptTensor& status) {
+                          Tensor& k_cache, Tensor& v_cache, int64_t Hq, int64_t Hkv, int64_t D, const OptTensor& status, const OptTensor& k_scale,
+                          const OptTensor& v_scale) {
+  if (k_cache.scalar_type() != torch::kBFloat16) {  // 8 bits
+    const char* op = "rope_kv_write_decode";
+    TORCH_CHECK(Hq >= 0 && Hkv > 0, op, ": heads");
+    cache_args::written_rows(qkv, (Hq + 2 * Hkv) * D, op, "qkv");
+    const torch::Device dev = qkv.device();
+    const int64_t B = qkv.size(0);
+    const agrpo::PagedCache c = cache_args::cache(k_cache, v_cache, k_scale, v_scale, dev, D, op);
+    TORCH_CHECK(c.Hkv == Hkv, op, ": cache of ", std::to_string(Hkv), " kv heads");
+    check_f32(cos_t, "cos"); check_f32(sin_t, "sin");
+    TORCH_CHECK(cos_t.device() == dev && sin_t.device() == dev && cos_t.dim() == 2 && cos_t.size(0) > 0 && cos_t.size(1) == D / 2 && cos_t.is_contiguous() &&
+                sin_t.is_contiguous() && sin_t.sizes() == cos_t.sizes() && cache_args::aligned16(cos_t) && cache_args::aligned16(sin_t), op,
+                ": tables [max_pos, D / 2], 16-byte aligned");
+    cache_args::ints(seq_lens, dev, B, op, "seq_lens");
+    TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.device() == dev && block_tables.dim() == 2 && block_tables.size(0) >= B &&
+                (block_tables.size(1) <= 1 || block_tables.stride(1) == 1), op, ": block_tables int32 [sequences, blocks], inner stride 1");
+    cache_args::status_word(status, dev, op);
+    const c10::cuda::CUDAGuard guard(dev);
+    agrpo::launch_rope_kv8_write_decode(qkv.data_ptr(), qkv.stride(0), cos_t.data_ptr<float>(), sin_t.data_ptr<float>(), (int)cos_t.size(0),
+                                        block_tables.data_ptr<int>(), block_tables.stride(0), (int)block_tables.size(1), seq_lens.data_ptr<int>(), c,
+                                        (int)B, (int)Hq, opt_ptr<int>(status), cur_stream());
+    return;
+  }
+  TORCH_CHECK(!cache_args::given(k_scale) && !cache_args::given(v_scale), "rope_kv_write_decode: a bf16 cache has no scales");
   check_bf16(qkv, "qkv"); check_f32(cos_t, "cos"); check_f32(sin_t, "sin"); check_i32(block_tables, "block_tables");
   check_i32(seq_lens, "seq_lens"); check_bf16(k_cache, "k_cache"); check_bf16(v_cache, "v_cache");
   TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(0) % 8 == 0, "rope_kv_write: qkv");
@@ -1220,6 +1260,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_property_readonly("num_cached_blocks", &agrpo::Scheduler::num_cached_blocks)
       .def("clear_prefix_cache", &agrpo::Scheduler::clear_prefix_cache);
 
+  bind_cache_ops(m);
   bind_layer_ops(m);
   bind_hybrid_ops(m);
   m.def("gemm_bf16", &gemm_bf16, py::arg("a"), py::arg("b"), py::arg("d"), py::arg("a_mn") = false,
@@ -1294,12 +1335,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dlogp"), py::arg("temperature"), py::arg("dz_chunk"), py::arg("dh_acc"), py::arg("dweight") = py::none(),
         py::arg("status") = py::none(), py::arg("logits") = py::none(), NOGIL);
   m.def("kv_cache_write", &kv_cache_write, py::arg("qkv"), py::arg("slots"), py::arg("k_cache"), py::arg("v_cache"), py::arg("Hq"),
-        py::arg("Hkv"), py::arg("D"), py::arg("status") = py::none(), py::arg("kv_head0") = 0, NOGIL);
+        py::arg("Hkv"), py::arg("D"), py::arg("status") = py::none(), py::arg("kv_head0") = 0, py::arg("k_scale") = py::none(),
+        py::arg("v_scale") = py::none(), NOGIL,
+        "k and v of the rows of `qkv` into their cache slots (negative: none). No slot may be named twice. The cache is bf16, or e4m3 with a scale "
+        "byte for each vector (k_scale, v_scale uint8 [blocks, heads, block size]).");
   m.def("kv_cache_write_decode", &kv_cache_write_decode, py::arg("qkv"), py::arg("block_tables"), py::arg("seq_lens"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("Hq"), py::arg("Hkv"), py::arg("D"), py::arg("status") = py::none(), NOGIL);
   m.def("rope_kv_write_decode", &rope_kv_write_decode, py::arg("qkv"), py::arg("cos"), py::arg("sin"), py::arg("block_tables"),
         py::arg("seq_lens"), py::arg("k_cache"), py::arg("v_cache"), py::arg("Hq"), py::arg("Hkv"), py::arg("D"),
-        py::arg("status") = py::none(), NOGIL);
+        py::arg("status") = py::none(), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(), NOGIL);
   m.def("paged_decode_attn", &paged_decode_attn, py::arg("qkv"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("block_tables"), py::arg("seq_lens"), py::arg("out"), py::arg("Hq"), py::arg("Hkv"), py::arg("D"),
         py::arg("softmax_scale"), py::arg("splits") = 1, py::arg("part_o") = py::none(), py::arg("part_ml") = py::none(),

@@ -3,3 +3,4 @@
 
 void bind_layer_ops(pybind11::module_& m);
 void bind_hybrid_ops(pybind11::module_& m);
+void bind_cache_ops(pybind11::module_& m);

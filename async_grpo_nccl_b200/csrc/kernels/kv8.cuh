@@ -1,0 +1,84 @@
+// The 8-bit form of a KV cache. A vector (the D values of one token and one kv head, of K or of V) is D e4m3 codes and one power of
+// two, 2^e, kept as the byte e + 127: the smallest with max|x| <= 448 * 2^e, and e >= -116. A vector that holds an infinity or a NaN
+// has byte 255 and reads as NaN.
+//
+// Why a power of two: dividing by it and multiplying with it round nothing, so a value is rounded once, to the 3 mantissa bits of its
+// code, and what a code stands for is exact in bf16. Attention over an 8-bit cache is then attention over the bf16 values that
+// kv_cache_read gives. A scale max|x| / 448 would use up to one binade more of e4m3's 15 for small values, at the price of a second rounding.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace agrpo {
+
+constexpr int kKv8MinByte = 11;   // e = -116: everything below is within half a step of zero
+constexpr int kKv8NanByte = 255;
+constexpr int kKv8TopByte = 247;  // e = 120: its codes above 240 would stand for 2^128
+
+// Scale byte of a vector whose largest magnitude has these bf16 bits (sign cleared; 448 = 1.75 * 2^8: mantissa 96 of 128).
+__device__ __forceinline__ int kv8_scale_byte(uint32_t top) {
+  if (top >= 0x7f80u) return kKv8NanByte;
+  return max(static_cast<int>(top >> 7) - 8 + ((top & 127u) > 96u ? 1 : 0), kKv8MinByte);
+}
+
+// Largest of the magnitudes of 8 bf16 values, as bits.
+__device__ __forceinline__ uint32_t kv8_top(const uint4& v) {
+  const uint32_t a = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  return max(a & 0xffffu, a >> 16);
+}
+
+// Codes of 8 bf16 values under a scale byte.
+__device__ __forceinline__ uint2 kv8_encode(const uint4& v, int byte) {
+  if (byte == kKv8NanByte) return make_uint2(0u, 0u);
+  const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
+  const float lim = byte >= kKv8TopByte ? 240.f : 448.f;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t half[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f = make_float2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+    f.x = fminf(fmaxf(f.x, -lim), lim);
+    f.y = fminf(fmaxf(f.y, -lim), lim);
+    half[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(half[0] | (half[1] << 16), half[2] | (half[3] << 16));
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Factors (both halves of a word) that turn codes moved into bf16's exponent field into what they stand for. An e4m3 code moved there is
+// 2^-120 of its value, subnormals included (bias 127 against 7); 2^120 * 2^e is a bf16 number up to e = 7, beyond that a second
+// factor follows.
+struct Kv8Scale {
+  uint32_t first, second;
+  bool twice;
+};
+__device__ __forceinline__ Kv8Scale kv8_scale(int byte) {
+  Kv8Scale s;
+  const uint32_t a = byte == kKv8NanByte ? 0x7fc0u : static_cast<uint32_t>(min(120 + byte, 254)) << 7;
+  s.first = a | (a << 16);
+  s.twice = byte > 134 && byte != kKv8NanByte;
+  const uint32_t b = static_cast<uint32_t>(byte - 7) << 7;
+  s.second = b | (b << 16);
+  return s;
+}
+// Four codes -> four bf16 values.
+__device__ __forceinline__ uint2 kv8_decode4(uint32_t codes, const Kv8Scale& s) {
+  uint32_t lo = __byte_perm(codes, 0u, 0x1404), hi = __byte_perm(codes, 0u, 0x3424);  // a code in the upper byte of each half
+  lo = (lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u);
+  hi = (hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u);
+  lo = mul_bf16x2(lo, s.first);
+  hi = mul_bf16x2(hi, s.first);
+  if (s.twice) {
+    lo = mul_bf16x2(lo, s.second);
+    hi = mul_bf16x2(hi, s.second);
+  }
+  return make_uint2(lo, hi);
+}
+
+}  // namespace agrpo

@@ -1,0 +1,204 @@
+// KV cache in 8 bits: written from the rows of a prefill, written by a decode step with its rotation, read back into rows.
+// All three move bytes: a vector of D bf16 values is 2 D bytes on one side and D + 1 on the other.
+#include <cuda_bf16.h>
+
+#include "../common/ptx.cuh"
+#include "../launchers.h"
+#include "../launchers_cache.h"
+#include "kv8.cuh"
+#include "rope.cuh"
+
+namespace agrpo {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Largest of the values of the `kLanes` lanes that share a vector.
+template <int kLanes>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// D / 8 lanes a vector, 16 bytes of bf16 each.
+template <int D>
+__global__ void __launch_bounds__(kThreads)
+kv8_write_kernel(const __nv_bfloat16* __restrict__ qkv, long long pitch, int k_col0, int v_col0, const int* __restrict__ slots, PagedCache c,
+                 long long vectors, int* status) {
+  constexpr int kLanes = D / 8;
+  const int lane = threadIdx.x % kLanes;
+  const long long vec = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  const int per_row = 2 * c.Hkv;
+  const bool on = vec < vectors;
+  const long long t = on ? vec / per_row : 0;
+  const int which = on ? static_cast<int>(vec - t * per_row) : 0;
+  const bool is_v = which >= c.Hkv;
+  const int h = is_v ? which - c.Hkv : which;
+  const int slot = on ? slots[t] : -1;
+  const bool bad = slot >= 0 && slot / c.block_size >= c.num_blocks;
+  if (bad && lane == 0) report_status(status, kStatusBadIndex);
+  const bool write = slot >= 0 && !bad;
+  uint4 x = make_uint4(0u, 0u, 0u, 0u);
+  if (write) x = *reinterpret_cast<const uint4*>(qkv + t * pitch + (is_v ? v_col0 : k_col0) + h * D + lane * 8);
+  const int byte = kv8_scale_byte(group_max<kLanes>(kv8_top(x)));
+  if (!write) return;
+  const long long at = (static_cast<long long>(slot / c.block_size) * c.Hkv + h) * c.block_size + slot % c.block_size;
+  uint8_t* codes = static_cast<uint8_t*>(is_v ? c.v : c.k) + at * D + lane * 8;
+  *reinterpret_cast<uint2*>(codes) = kv8_encode(x, byte);
+  if (lane == 0) (is_v ? c.v_scale : c.k_scale)[at] = static_cast<uint8_t>(byte);
+}
+
+// D / 16 lanes a vector: 16 codes (or 32 bytes of bf16) each.
+template <int D, bool k8>
+__global__ void __launch_bounds__(kThreads)
+kv_cache_read_kernel(PagedCache c, const int* __restrict__ slots, __nv_bfloat16* __restrict__ qkv, long long pitch, int k_col0, int v_col0,
+                     long long vectors, int* status) {
+  constexpr int kLanes = D / 16;
+  const int lane = threadIdx.x % kLanes;
+  const long long vec = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  if (vec >= vectors) return;
+  const int per_row = 2 * c.Hkv;
+  const long long t = vec / per_row;
+  const int which = static_cast<int>(vec - t * per_row);
+  const bool is_v = which >= c.Hkv;
+  const int h = is_v ? which - c.Hkv : which;
+  const int slot = slots[t];
+  if (slot < 0) return;
+  if (slot / c.block_size >= c.num_blocks) {
+    if (lane == 0) report_status(status, kStatusBadIndex);
+    return;
+  }
+  const long long at = (static_cast<long long>(slot / c.block_size) * c.Hkv + h) * c.block_size + slot % c.block_size;
+  uint4* dst = reinterpret_cast<uint4*>(qkv + t * pitch + (is_v ? v_col0 : k_col0) + h * D + lane * 16);
+  const void* src = is_v ? c.v : c.k;
+  if (k8) {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + at * D + lane * 16);
+    const Kv8Scale s = kv8_scale((is_v ? c.v_scale : c.k_scale)[at]);
+    const uint2 a = kv8_decode4(w.x, s), b = kv8_decode4(w.y, s), d = kv8_decode4(w.z, s), e = kv8_decode4(w.w, s);
+    dst[0] = make_uint4(a.x, a.y, b.x, b.y);
+    dst[1] = make_uint4(d.x, d.y, e.x, e.y);
+  } else {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(src) + at * D + lane * 16);
+    const uint4 a = p[0], b = p[1];
+    dst[0] = a;
+    dst[1] = b;
+  }
+}
+
+// One CTA a row; D / 16 lanes a head, each with 8 values of the lower half of the head and the 8 that they are rotated with. The rotated
+// key is rounded to bf16, as the row keeps it, before it is quantised: a token's entry is the same from a decode step as from a prefill.
+template <int D>
+__global__ void __launch_bounds__(128)
+rope_kv8_write_decode_kernel(__nv_bfloat16* __restrict__ qkv, long long pitch, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
+                             int max_pos, const int* __restrict__ block_tables, long long table_pitch, int max_blocks,
+                             const int* __restrict__ seq_lens, PagedCache c, int Hq, int* status) {
+  pdl_wait();
+  pdl_launch();
+  constexpr int kLanes = D / 16, kHalf = D / 2;
+  const int b = blockIdx.x, lane = threadIdx.x % kLanes;
+  const int len = seq_lens[b];
+  const int pos = len > 0 ? len - 1 : 0;
+  const int p = pos >= max_pos ? max_pos - 1 : pos;
+  int blk = -1;
+  if (len > 0) {
+    blk = pos / c.block_size < max_blocks ? block_tables[b * table_pitch + pos / c.block_size] : -1;
+    if (blk < 0 || blk >= c.num_blocks) {
+      if (threadIdx.x == 0) report_status(status, kStatusBadIndex);
+      blk = -1;
+    }
+  }
+  const int heads = Hq + 2 * c.Hkv;
+  const int per = 128 / kLanes;
+  for (int h0 = 0; h0 < heads; h0 += per) {
+    const int h = h0 + threadIdx.x / kLanes;
+    const bool on = h < heads, is_v = h >= Hq + c.Hkv;
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+    uint4* x = reinterpret_cast<uint4*>(qkv + b * pitch + static_cast<long long>(h) * D + lane * 8);
+    if (on) {
+      lo = x[0];
+      hi = x[kHalf / 8];
+    }
+    if (on && !is_v) {
+      const float* cr = cos_t + static_cast<long long>(p) * kHalf + lane * 8;
+      const float* sr = sin_t + static_cast<long long>(p) * kHalf + lane * 8;
+      float cv[8], sv[8];
+      *reinterpret_cast<float4*>(cv) = *reinterpret_cast<const float4*>(cr);
+      *reinterpret_cast<float4*>(cv + 4) = *reinterpret_cast<const float4*>(cr + 4);
+      *reinterpret_cast<float4*>(sv) = *reinterpret_cast<const float4*>(sr);
+      *reinterpret_cast<float4*>(sv + 4) = *reinterpret_cast<const float4*>(sr + 4);
+      uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+      uint32_t* u = reinterpret_cast<uint32_t*>(&hi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float a0 = __uint_as_float(l[i] << 16), a1 = __uint_as_float(l[i] & 0xffff0000u);
+        float b0 = __uint_as_float(u[i] << 16), b1 = __uint_as_float(u[i] & 0xffff0000u);
+        rope_rotate(a0, b0, cv[2 * i], sv[2 * i]);
+        rope_rotate(a1, b1, cv[2 * i + 1], sv[2 * i + 1]);
+        l[i] = pack_bf16x2(a0, a1);
+        u[i] = pack_bf16x2(b0, b1);
+      }
+      x[0] = lo;
+      x[kHalf / 8] = hi;
+    }
+    const int byte = kv8_scale_byte(group_max<kLanes>(max(kv8_top(lo), kv8_top(hi))));
+    if (!on || h < Hq || blk < 0) continue;
+    const int kh = is_v ? h - Hq - c.Hkv : h - Hq;
+    const long long at = (static_cast<long long>(blk) * c.Hkv + kh) * c.block_size + pos % c.block_size;
+    uint8_t* codes = static_cast<uint8_t*>(is_v ? c.v : c.k) + at * D + lane * 8;
+    *reinterpret_cast<uint2*>(codes) = kv8_encode(lo, byte);
+    *reinterpret_cast<uint2*>(codes + kHalf) = kv8_encode(hi, byte);
+    if (lane == 0) (is_v ? c.v_scale : c.k_scale)[at] = static_cast<uint8_t>(byte);
+  }
+}
+
+}  // namespace
+
+void launch_kv8_write(const void* qkv, long long pitch, int k_col0, int v_col0, const int* slots, const PagedCache& c, int T, int* status,
+                      cudaStream_t s) {
+  const long long vectors = static_cast<long long>(T) * 2 * c.Hkv;
+  if (vectors == 0) return;
+  const int lanes = c.D / 8;
+  const unsigned blocks = static_cast<unsigned>((vectors * lanes + kThreads - 1) / kThreads);
+  const auto run = [&](auto kernel) {
+    kernel<<<blocks, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(qkv), pitch, k_col0, v_col0, slots, c, vectors, status);
+    check_cuda(cudaGetLastError(), "kv8_write");
+  };
+  if (c.D == 128) run(kv8_write_kernel<128>);
+  else run(kv8_write_kernel<64>);
+}
+
+void launch_kv_cache_read(const PagedCache& c, const int* slots, void* qkv, long long pitch, int k_col0, int v_col0, int T, int* status,
+                          cudaStream_t s) {
+  const long long vectors = static_cast<long long>(T) * 2 * c.Hkv;
+  if (vectors == 0) return;
+  const int lanes = c.D / 16;
+  const unsigned blocks = static_cast<unsigned>((vectors * lanes + kThreads - 1) / kThreads);
+  const auto run = [&](auto kernel) {
+    kernel<<<blocks, kThreads, 0, s>>>(c, slots, static_cast<__nv_bfloat16*>(qkv), pitch, k_col0, v_col0, vectors, status);
+    check_cuda(cudaGetLastError(), "kv_cache_read");
+  };
+  const bool k8 = c.k_scale != nullptr;
+  if (c.D == 128) k8 ? run(kv_cache_read_kernel<128, true>) : run(kv_cache_read_kernel<128, false>);
+  else k8 ? run(kv_cache_read_kernel<64, true>) : run(kv_cache_read_kernel<64, false>);
+}
+
+void launch_rope_kv8_write_decode(void* qkv, long long pitch, const float* cos_t, const float* sin_t, int max_pos, const int* block_tables,
+                                  long long table_pitch, int max_blocks, const int* seq_lens, const PagedCache& c, int B, int Hq, int* status,
+                                  cudaStream_t s) {
+  if (B == 0) return;
+  const auto run = [&](auto kernel) {
+    launch_kernel(kernel, dim3(B), dim3(128), 0, s, "rope_kv8_write_decode", static_cast<__nv_bfloat16*>(qkv), pitch, cos_t, sin_t, max_pos,
+                  block_tables, table_pitch, max_blocks, seq_lens, c, Hq, status);
+  };
+  if (c.D == 128) {
+    AGRPO_PREFER_SMEM(rope_kv8_write_decode_kernel<128>);
+    run(rope_kv8_write_decode_kernel<128>);
+  } else {
+    AGRPO_PREFER_SMEM(rope_kv8_write_decode_kernel<64>);
+    run(rope_kv8_write_decode_kernel<64>);
+  }
+}
+
+}  // namespace agrpo

@@ -196,3 +196,53 @@ def stats_to_metrics(stats: Sequence[float], loss_value: float, num_samples: int
         "dual_clip_frac": s["dual_clip"] / n,
         "num_tokens": s["count"],
     }
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# paged cache, 8 bits
+# ---------------------------------------------------------------------------------------------------------------------
+KV8_MIN_BYTE, KV8_NAN_BYTE, KV8_TOP_BYTE = 11, 255, 247
+
+
+def kv8_quantise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 codes, scale bytes) of the vectors along the last dimension of ``x``: 2^e is the smallest power of two, e >= -116, with
+    max|x| <= 448 * 2^e; the byte is e + 127. 255 marks a vector that holds an infinity or a NaN."""
+    x = x.double()
+    fine = torch.isfinite(x).all(-1)
+    x = torch.where(fine[..., None], x, torch.zeros_like(x))
+    m, e = torch.frexp(x.abs().amax(-1).clamp(min=2.0 ** -126))
+    e = torch.clamp(e - 9 + (m > 0.875).to(e.dtype), min=KV8_MIN_BYTE - 127)  # 448 = 0.875 * 2^9
+    byte = torch.where(fine, e + 127, torch.full_like(e, KV8_NAN_BYTE))
+    y = torch.ldexp(x, -e[..., None])
+    top = torch.where(byte >= KV8_TOP_BYTE, 240.0, 448.0)[..., None].to(y.dtype)  # the next code would stand for 2^128
+    y = torch.minimum(torch.maximum(y, -top), top)
+    return y.float().to(torch.float8_e4m3fn), byte.to(torch.uint8)
+
+
+def kv8_values(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """What the codes stand for (fp64; exact in bf16)."""
+    v = torch.ldexp(codes.float().double(), scale.to(torch.int32)[..., None] - 127)
+    return torch.where((scale == KV8_NAN_BYTE)[..., None], torch.full_like(v, math.nan), v)
+
+
+def paged_chunk_attention(qkv, k, v, block_tables, seq_lens, q_starts, Hq, Hkv, D, softmax_scale):
+    """fp64 attention of every sequence's newest rows over its pages (k, v: values [blocks, Hkv, block size, D]). Returns ([rows, Hq * D],
+    sum_k p |v| likewise, for error bounds)."""
+    out = torch.zeros(qkv.shape[0], Hq, D, dtype=torch.float64, device=qkv.device)
+    size = torch.zeros_like(out)
+    bs, G = k.shape[2], Hq // Hkv
+    starts = q_starts.tolist()
+    for b, total in enumerate(seq_lens.tolist()[:len(starts) - 1]):
+        a, z = starts[b], starts[b + 1]
+        if a == z or total == 0:
+            continue
+        pages = block_tables[b, :(total + bs - 1) // bs].long()
+        kk, vv = (c[pages].transpose(0, 1).reshape(Hkv, -1, D)[:, :total].double() for c in (k, v))
+        q = qkv[a:z, :Hq * D].double().view(z - a, Hkv, G, D)
+        s = torch.einsum("nhgd,hld->hgnl", q, kk) * softmax_scale
+        see = torch.arange(total, device=s.device)[None] <= torch.arange(z - a, device=s.device)[:, None] + (total - (z - a))
+        s = s.masked_fill(~see, -math.inf)
+        p = torch.softmax(s, -1).masked_fill(~see, 0.0)  # a row that sees nothing is zero
+        out[a:z] = torch.einsum("hgnl,hld->nhgd", p, vv).reshape(z - a, Hq, D)
+        size[a:z] = torch.einsum("hgnl,hld->nhgd", p, vv.abs()).reshape(z - a, Hq, D)
+    return out.flatten(1), size.flatten(1)

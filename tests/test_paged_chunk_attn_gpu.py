@@ -1,0 +1,263 @@
+"""Attention of new tokens over the paged cache against 64 bits.
+
+Tolerance: bf16 results are off by 2^-8 of their value, the probabilities, rounded to bf16 for the second product, by 2^-8 each, which adds at
+most 2^-8 sum p|v|. What is left is fp32: a logit of 128 products is off by less than 2^-16 here (|q.k| s log2 e summed by magnitude is below 2^6),
+the exponential and the running sums by 2^-20 and a few thousand times 2^-24; 2^-10 sum p|v| covers them."""
+import math
+
+import pytest
+import torch
+
+from async_grpo_nccl_b200.ops import reference as R
+from gpu_util import native, status_word
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+# (new rows, tokens in the cache): single tokens around the tiles' edges, idle and empty ones, rows that see nothing, chunks
+MIXED = [(1, 1), (1, 0), (0, 5), (0, 0), (3, 2), (1, 127), (1, 128), (1, 129), (17, 17), (2, 700), (130, 1000), (257, 300), (5, 0), (1, 2049)]
+
+
+class Case:
+    def __init__(self, seqs, Hq, Hkv, D, bs, eight, pad=0, pitch=0, seed=0, q_scale=1.5):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.Hq, self.Hkv, self.D, self.bs = Hq, Hkv, D, bs
+        per = [-(-L // bs) for _, L in seqs]
+        blocks = sum(per) + 2
+        order = torch.randperm(blocks, device=DEV, generator=g).int().tolist()
+        width = max(1, max(per))
+        self.table = torch.full((len(seqs), width + 3), 2 ** 30, dtype=torch.int32, device=DEV)[:, :width]  # entries behind a sequence mean nothing
+        at, kv = 0, [torch.randn(blocks, Hkv, bs, D, device=DEV, generator=g).bfloat16() + i for i in range(2)]
+        held = torch.zeros(blocks, bs, dtype=torch.bool, device=DEV)
+        for b, n in enumerate(per):
+            pages = order[at:at + n]
+            at += n
+            if n:
+                self.table[b, :n] = torch.tensor(pages, dtype=torch.int32, device=DEV)
+                held.view(-1)[(torch.tensor(pages, device=DEV)[:, None] * bs + torch.arange(bs, device=DEV)).reshape(-1)[:seqs[b][1]]] = True
+        self.scales = [None, None]
+        if eight:
+            both = [R.kv8_quantise(c.float()) for c in kv]
+            self.values = [R.kv8_values(*b) for b in both]
+            kv, self.scales = [b[0] for b in both], [b[1] for b in both]
+            for c, s in zip(kv, self.scales):
+                c.view(torch.uint8).masked_fill_(~held[:, None, :, None], 0x7f)  # NaN where no sequence has a token
+                s.masked_fill_(~held[:, None], 255)
+        else:
+            self.values = [c.clone() for c in kv]
+            for c in kv:
+                c.masked_fill_(~held[:, None, :, None], math.nan)
+        self.kv = kv
+        n = [a for a, _ in seqs]
+        self.Tq = sum(n) + pad
+        self.rows = (torch.randn(self.Tq, (Hq + 2 * Hkv) * D + pitch, device=DEV, generator=g) * q_scale).bfloat16()[:, :(Hq + 2 * Hkv) * D]
+        self.starts = torch.tensor([0] + n, device=DEV).cumsum(0).int()
+        self.lens = torch.tensor([b for _, b in seqs], device=DEV).int()
+        self.out = torch.full((self.Tq, Hq * D + pitch), 7.0, device=DEV, dtype=torch.bfloat16)[:, :Hq * D]
+        self.status = status_word()
+
+    def call(self, **kw):
+        a = dict(status=self.status, k_scale=self.scales[0], v_scale=self.scales[1])
+        a.update(kw)
+        native().paged_chunk_attn(self.rows, self.kv[0], self.kv[1], self.table, self.lens, self.starts, self.out, self.Hq, self.Hkv, self.D,
+                                  1 / math.sqrt(self.D), **a)
+
+    def check(self):
+        want, size = R.paged_chunk_attention(self.rows, self.values[0], self.values[1], self.table, self.lens, self.starts, self.Hq, self.Hkv, self.D,
+                                             1 / math.sqrt(self.D))
+        n = int(self.starts[-1])
+        off = (self.out[:n].double() - want[:n]).abs() - (want[:n].abs() * 2.0 ** -8 + size[:n] * (2.0 ** -8 + 2.0 ** -10))
+        assert bool(self.out[:n].isfinite().all())
+        assert n == 0 or float(off.max()) <= 0, (float(off.max()), torch.nonzero(off > 0)[:8].tolist())
+        assert bool((self.out[n:] == 7).all())
+        assert int(self.status) == 0
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D,bs", [(12, 2, 128, 16), (28, 4, 128, 16), (5, 1, 64, 16), (8, 8, 128, 32), (64, 2, 128, 16), (14, 2, 64, 64), (3, 3, 64, 128),
+                                         (16, 2, 128, 128)])
+def test_mixed_lengths(Hq, Hkv, D, bs, eight):
+    c = Case(MIXED, Hq, Hkv, D, bs, eight, pad=3, pitch=64, seed=Hq)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("seqs", [[(1, 1)], [(1, 700)], [(1, 40000)], [(4, 4)], [(1, 50)] * 300, [(1, L) for L in range(0, 400, 3)], [(7, 3000)] * 9, [(1000, 1000)],
+                                  [(333, 5000), (1, 9)], [(64, 64 + i) for i in range(40)], [(0, 3)] * 5 + [(1, 3)], [(2100, 2100), (0, 0), (1500, 1777)],
+                                  [(1, 5000)] * 150])
+def test_uses(seqs, eight):
+    """Decode steps, drafts, prompts and portions at one layout each."""
+    c = Case(seqs, 12, 2, 128, 16, eight, seed=len(seqs))
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("n", [1, 40])
+def test_large_logits(n, eight):
+    """Softmax over one or two keys of thousands: logits of several hundred, maxima that keep growing along the sequence."""
+    c = Case([(n, 3000)], 6, 1, 128, 16, eight, seed=n, q_scale=1.5)
+    big = 1 + 8 * torch.arange(c.kv[0].shape[0] * 16, device=DEV).float().view(-1, 1, 16, 1) / (c.kv[0].shape[0] * 16)
+    vals = (c.values[0].float() * big).bfloat16()
+    if eight:
+        codes, s = R.kv8_quantise(vals.float())
+        c.kv[0], c.scales[0], c.values[0] = codes, s, R.kv8_values(codes, s)
+    else:
+        c.kv[0] = c.values[0] = vals
+    c.call()
+    c.check()
+
+
+def test_a_sequence_does_not_depend_on_where_its_pages_are():
+    a = Case([(5, 700), (300, 900)], 12, 2, 128, 16, False, seed=1)
+    a.call()
+    blocks = a.kv[0].shape[0]
+    perm = torch.randperm(blocks, device=DEV)
+    first = a.out.clone()
+    a.kv = [torch.empty_like(c).index_copy_(0, perm, c) for c in a.kv]
+    inside = a.table < blocks
+    a.table[inside] = perm[a.table[inside].long()].int()
+    a.out.fill_(7)
+    a.call()
+    assert torch.equal(a.out, first)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_the_same_call_gives_the_same_bits(eight):
+    c = Case([(1, 3000)] * 20 + [(200, 2000)], 12, 2, 128, 16, eight)
+    c.call()
+    first = c.out.clone()
+    for _ in range(5):
+        c.out.fill_(7)
+        c.call()
+        assert torch.equal(c.out, first)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_captured_calls_follow_the_lengths(eight):
+    """Two graphs captured one after the other, replayed in turn on two streams with other lengths than at capture, beside an eager call."""
+    cases = [Case([(1, 900), (1, 300), (1, 40)], 12, 2, 128, 16, eight, seed=3), Case([(60, 1500), (3, 700)], 12, 2, 128, 16, eight, seed=4)]
+    graphs = []
+    for c in cases:
+        c.call()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.call()
+        graphs.append(g)
+    cases[0].lens.copy_(torch.tensor([17, 300, 0]))
+    cases[1].lens.copy_(torch.tensor([1300, 3]))
+    eager = Case([(1, 2000)] * 7, 12, 2, 128, 16, eight, seed=5)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s, f in zip(streams, (graphs[0].replay, graphs[1].replay, eager.call)):
+            with torch.cuda.stream(s):
+                f()
+    torch.cuda.synchronize()
+    for c in cases + [eager]:
+        c.check()
+
+
+def test_pages_and_lengths_that_do_not_exist_are_reported():
+    for page in (-1, 10 ** 6):
+        c = Case([(1, 100), (1, 100)], 12, 2, 128, 16, False)
+        c.table[0, 2] = page
+        c.call()
+        assert int(c.status) == 6
+        c.status.zero_()
+        want = c.out[1].clone()
+        c.table[0, 2] = c.table[1, 0]
+        c.call()
+        assert int(c.status) == 0 and torch.equal(c.out[1], want)
+    c = Case([(1, 100), (1, 50)], 12, 2, 128, 16, True)
+    c.lens[0] = 2 ** 30  # more than its table holds
+    c.call()
+    assert int(c.status) == 6
+    c = Case([(1, 100), (2, 50)], 12, 2, 128, 16, True)
+    for bad in ([0, 9, 3], [0, 2, 1], [-5, 1, 3]):  # starts that leave the rows or go back
+        c.status.zero_()
+        c.out.fill_(7)
+        c.starts.copy_(torch.tensor(bad))
+        c.call()
+        assert int(c.status) == 6
+
+
+def test_a_cache_behind_two_gigabytes():
+    Hkv, D, bs = 8, 128, 16
+    blocks = (1 << 31) // (Hkv * D * bs) + 40
+    c = Case([(1, 300), (9, 200)], 16, Hkv, D, bs, True)
+    n = c.kv[0].shape[0]
+    k, v = (torch.empty(blocks, Hkv, bs, D, dtype=torch.uint8, device=DEV) for _ in range(2))
+    s = [torch.zeros(blocks, Hkv, bs, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    for big, small, sb, ss in zip((k, v), c.kv, s, c.scales):
+        big[-n:] = small.view(torch.uint8)
+        sb[-n:] = ss
+    c.call()
+    first = c.out.clone()
+    c.kv, c.scales = [k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn)], s
+    c.table += blocks - n
+    c.out.fill_(7)
+    c.call()
+    assert torch.equal(c.out, first) and int(c.status) == 0
+
+
+def test_the_cache_that_was_written_is_what_is_attended():
+    """Operators in a row, as an engine runs them: rows written in 8 bits, attended in place, and the same over what is read back."""
+    C = native()
+    Hq, Hkv, D, bs, T = 12, 2, 128, 16, 333
+    c = Case([(T, T)], Hq, Hkv, D, bs, True)
+    slots = (c.table[0, :, None] * bs + torch.arange(bs, device=DEV)).reshape(-1)[:T].int().contiguous()
+    C.kv_cache_write(c.rows, slots, c.kv[0], c.kv[1], Hq, Hkv, D, c.status, 0, c.scales[0], c.scales[1])
+    both = c.rows.float().view(T, Hq + 2 * Hkv, D)[:, Hq:]
+    for i in range(2):
+        c.values[i] = c.values[i].clone()
+        c.values[i].transpose(1, 2).reshape(-1, Hkv, D)
+        flat = c.values[i].transpose(1, 2).reshape(-1, Hkv, D).clone()
+        flat[slots.long()] = R.kv8_values(*R.kv8_quantise(both[:, i * Hkv:(i + 1) * Hkv]))
+        c.values[i] = flat.view(-1, bs, Hkv, D).transpose(1, 2)
+    c.call()
+    c.check()
+    back = c.rows.clone()
+    C.kv_cache_read(c.kv[0], c.kv[1], slots, back, Hq, Hkv, D, c.status, c.scales[0], c.scales[1])
+    k, v = (torch.zeros(c.kv[0].shape, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    C.kv_cache_write(back, slots, k, v, Hq, Hkv, D, c.status)
+    eight = c.out.clone()
+    c.kv, c.scales = [k, v], [None, None]
+    c.call()
+    c.check()
+    assert torch.equal(c.out, eight)  # the same values, the same products
+
+
+def test_refusals():
+    c = Case([(2, 40)], 12, 2, 128, 16, True)
+
+    def refused(match, **kw):
+        a = dict(qkv=c.rows, k=c.kv[0], v=c.kv[1], table=c.table, lens=c.lens, starts=c.starts, out=c.out, Hq=12, Hkv=2, D=128, ks=c.scales[0], vs=c.scales[1])
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            native().paged_chunk_attn(a["qkv"], a["k"], a["v"], a["table"], a["lens"], a["starts"], a["out"], a["Hq"], a["Hkv"], a["D"], 0.1, c.status, a["ks"], a["vs"])
+
+    refused("head_dim", D=96)
+    refused("1 to 32", Hq=13)
+    refused("1 to 32", Hq=128)
+    refused("cache of", Hq=4, Hkv=4, out=c.out[:, :512])
+    refused("cache of|heads of this rank", Hkv=1)
+    refused("needs k_scale", ks=None)
+    refused("scales uint8", vs=c.scales[1][:1])
+    refused("out \\[rows", out=c.out[:1])
+    refused("out bf16", out=c.out.float())
+    refused("must not be qkv", out=c.rows[:, :1536])
+    refused("rows overlap", out=c.out[:1].expand(2, -1))
+    refused("q_starts int32", starts=c.starts.long())
+    refused("seq_lens int32", lens=c.lens[:0])
+    refused("block_tables", table=c.table.long())
+    refused("block_tables", table=c.table[:0])
+    refused("on the device", lens=c.lens.cpu())
+    small = torch.zeros(4, 2, 8, 128, dtype=torch.float8_e4m3fn, device=DEV)
+    sc = torch.zeros(4, 2, 8, dtype=torch.uint8, device=DEV)
+    refused("block size", k=small, v=small, ks=sc, vs=sc)
+    # nothing to do
+    native().paged_chunk_attn(c.rows[:0], c.kv[0], c.kv[1], c.table[:0], c.lens[:0], c.starts[:1], c.out[:0], 12, 2, 128, 0.1, c.status, c.scales[0], c.scales[1])
+    assert bool((c.out == 7).all()) and int(c.status) == 0
