@@ -1207,6 +1207,8 @@ py::dict decode_plan_to_dict(const agrpo::DecodePlan& p) {
 }
 }  // namespace
 
+int launch_num_sms() { return num_sms(); }
+
 // Kernel launchers run without the interpreter lock: the trainer, logprob and rollout threads of one process launch
 // concurrently, and a decode step must not wait for another thread's launch sequence to yield.
 #define NOGIL py::call_guard<py::gil_scoped_release>()

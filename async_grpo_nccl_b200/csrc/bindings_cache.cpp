@@ -4,6 +4,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cmath>
+
 #include "bindings_layers.h"
 #include "launchers.h"
 
@@ -46,6 +48,8 @@ void paged_chunk_attn(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_
   TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.device() == dev && block_tables.dim() == 2 && block_tables.size(0) >= B &&
                   (block_tables.size(1) <= 1 || block_tables.stride(1) == 1), op, ": block_tables int32 [sequences, blocks], inner stride 1");
   TORCH_CHECK(B <= 8192 && block_tables.size(1) * c.block_size < (int64_t(1) << 30), op, ": at most 8192 sequences of 2^30 tokens");
+  TORCH_CHECK(std::isfinite(softmax_scale) && softmax_scale > 0, op, ": softmax_scale must be positive");
+  for (const OptTensor* s : {&k_scale, &v_scale}) TORCH_CHECK(!given(*s) || aligned16(**s), op, ": scales must be 16-byte aligned");
   status_word(status, dev, op);
   const c10::cuda::CUDAGuard guard(dev);
   agrpo::ChunkAttnArgs a;
@@ -63,7 +67,12 @@ void paged_chunk_attn(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_
   a.Hq = (int)Hq;
   a.softmax_scale = (float)softmax_scale;
   a.status = int_ptr(status);
-  agrpo::launch_paged_chunk_attn(a, c, at::cuda::getCurrentCUDAStream());
+  if (a.Tq == 0 || a.B == 0) return;
+  if (a.Tq == 1) a.ldq = Hq * D;  // the pitch of a single row means nothing
+  // Parts of units that several CTAs share: from the allocator, so that calls on several streams or in several graphs do not meet in it.
+  const int sms = launch_num_sms();
+  const Tensor scratch = at::empty({agrpo::paged_chunk_attn_scratch(a, c, sms)}, qkv.options().dtype(torch::kUInt8));
+  agrpo::launch_paged_chunk_attn(a, c, sms, scratch.data_ptr(), at::cuda::getCurrentCUDAStream());
 }
 
 }  // namespace

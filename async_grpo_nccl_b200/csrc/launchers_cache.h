@@ -39,6 +39,8 @@ struct ChunkAttnArgs {
   float softmax_scale;
   int* status;
 };
-void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, cudaStream_t s);
+// `scratch` holds paged_chunk_attn_scratch bytes, 16-byte aligned, and belongs to the call.
+long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, int num_sms);
+void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int num_sms, void* scratch, cudaStream_t s);
 
 }  // namespace agrpo
