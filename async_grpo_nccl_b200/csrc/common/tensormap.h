@@ -82,16 +82,25 @@ inline CUtensorMap make_tmap_2d(const void* base, uint64_t inner, uint64_t outer
   return m;
 }
 
-// 3-D bf16 map with 128-byte swizzle: dims[0] contiguous elements, pitches ld1 and ld2 (elements) of the outer two. box[0] = 64 elements.
-inline CUtensorMap make_tmap_3d(const void* base, const uint64_t (&dims)[3], uint64_t ld1, uint64_t ld2, const uint32_t (&box)[3]) {
+// Map of `rank` dimensions (3 to 5) over bf16 with 128-byte swizzle: dims[0] = box[0] = 64 elements, contiguous; pitch[i] elements from one index of
+// dimension i + 1 to the next.
+template <int kRank>
+inline CUtensorMap make_tmap_nd(const void* base, const uint64_t (&dims)[kRank], const uint64_t (&pitch)[kRank - 1], const uint32_t (&box)[kRank]) {
+  static_assert(kRank >= 3 && kRank <= 5, "rank");
   if ((reinterpret_cast<uint64_t>(base) & 15) != 0) throw std::runtime_error("TMA base address must be 16-byte aligned");
-  if (ld1 % 8 != 0 || ld2 % 8 != 0) throw std::runtime_error("TMA pitch must be a multiple of 16 bytes");
   CUtensorMap m;
-  cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
-  cuuint64_t strides[2] = {ld1 * 2, ld2 * 2};
-  cuuint32_t b[3] = {box[0], box[1], box[2]};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = get_encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), d, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t d[kRank], strides[kRank - 1];
+  cuuint32_t b[kRank], one[kRank];
+  for (int i = 0; i < kRank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    one[i] = 1;
+    if (i + 1 < kRank) {
+      if (pitch[i] % 8 != 0) throw std::runtime_error("TMA pitch must be a multiple of 16 bytes");
+      strides[i] = pitch[i] * 2;
+    }
+  }
+  CUresult r = get_encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRank, const_cast<void*>(base), d, strides, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
   return m;

@@ -32,6 +32,10 @@ namespace agrpo {
 namespace {
 
 constexpr int kBN = 128;  // keys a tile
+// A bf16 tile of keys in shared memory: 8 rows of 128 bytes (64 columns, swizzled) are an atom, an 8-row group holds its D / 64 atoms side by side.
+// So a whole page is one copy, whatever its length, and both products find equal strides between groups.
+template <int D>
+constexpr int kGroupBytes = D / 64 * 1024;
 constexpr int kSmemLimit = 232448;
 
 template <int D, bool k8, bool kFew>
@@ -309,8 +313,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int* table = p.a.block_tables + w.b * p.a.table_pitch;
       const int keys = unit_keys(p, w.s, w.qb);
       const int bs = p.c.block_size;
-      const int per_page = k8 ? 1 : kChunks;
-      const int page_of_lane = k8 ? lane & 15 : lane / per_page;
+      const int page_of_lane = k8 ? lane & 15 : lane;
       const auto page_id = [&](int j) {
         const int key = j * kBN + page_of_lane * bs;
         int id = page_of_lane * bs < kBN && key < keys ? table[key / bs] : 0;
@@ -340,15 +343,13 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           __syncwarp();
           if (page_of_lane < pages) {
             if (k8) {
-              const long long at_row = row;
               if (lane < 16) {
-                bulk_load_g2s(raw + slot * S::kRawBytes + page_of_lane * bs * D, static_cast<const uint8_t*>(v ? p.c.v : p.c.k) + at_row * D, bs * D, f);
+                bulk_load_g2s(raw + slot * S::kRawBytes + page_of_lane * bs * D, static_cast<const uint8_t*>(v ? p.c.v : p.c.k) + row * D, bs * D, f);
               } else {
-                bulk_load_g2s(raw_scale + slot * kBN + page_of_lane * bs, (v ? p.c.v_scale : p.c.k_scale) + at_row, bs, f);
+                bulk_load_g2s(raw_scale + slot * kBN + page_of_lane * bs, (v ? p.c.v_scale : p.c.k_scale) + row, bs, f);
               }
             } else {
-              const int ch = lane % per_page;
-              tma_load_2d(ring + slot * S::kSlotBytes + ch * (kBN * 128) + page_of_lane * bs * 128, v ? &tmV : &tmK, f, ch * 64, static_cast<int>(row));
+              tma_load_4d(ring + slot * S::kSlotBytes + page_of_lane * (bs / 8) * kGroupBytes<D>, v ? &tmV : &tmK, f, 0, 0, 0, static_cast<int>(row >> 3));
             }
           }
         }
@@ -394,8 +395,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const uint32_t q = aQ + t * (128 * D * 2), k = aRing + (item % S::kSlots) * S::kSlotBytes;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          const uint32_t off = (i / 4) * (128 * 128) + (i % 4) * 32;
-          tc_mma_f16(tmem + col, umma_smem_desc(q + off, 16, 1024), umma_smem_desc(k + off, 16, 1024), kIdescS, i > 0 ? 1u : 0u);
+          tc_mma_f16(tmem + col, umma_smem_desc(q + (i / 4) * (128 * 128) + (i % 4) * 32, 16, 1024),
+                     umma_smem_desc(k + (i / 4) * 1024 + (i % 4) * 32, 16, kGroupBytes<D>), kIdescS, i > 0 ? 1u : 0u);
         }
         tc_commit(s_full + (col >> 7));
       }
@@ -406,7 +407,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const uint32_t v = aRing + (item % S::kSlots) * S::kSlotBytes;
 #pragma unroll
         for (int i = 0; i < kBN / 16; ++i)
-          tc_mma_f16_ts(tmem + col_o, tmem + col_p + i * 8, umma_smem_desc(v + i * 2048, kBN * 128, 1024), kIdescO, (!first || i > 0) ? 1u : 0u);
+          tc_mma_f16_ts(tmem + col_o, tmem + col_p + i * 8, umma_smem_desc(v + i * 2 * kGroupBytes<D>, 1024, kGroupBytes<D>), kIdescO, (!first || i > 0) ? 1u : 0u);
       }
       __syncwarp();
     };
@@ -418,9 +419,9 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     const auto clear_tail = [&](int item, int valid) {
       if (k8 || valid >= kBN) return;
       uint8_t* v = ring + (item % S::kSlots) * S::kSlotBytes;
-      for (int i = max(valid, 0) * 8 + lane; i < kBN * 8; i += 32) {
+      for (int i = max(valid, 0) * 8 + lane; i < kBN * 8; i += 32) {  // row i / 8, bytes (i % 8) * 16 of its atoms
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(v + c * (kBN * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(v + (i >> 6) * kGroupBytes<D> + c * 1024 + (i & 63) * 16) = make_uint4(0u, 0u, 0u, 0u);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -491,8 +492,9 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     }
   } else if (k8 && warp >= S::kConvWarp) {
     // ---------------------------------------------------------------- 8 bits to bf16
-    // 16 codes a thread and step. Eight lanes take four pieces of a row and the other four of the next one: their 16-byte reads and writes
-    // fall into eight different bank groups.
+    // 16 codes a thread and step. A warp has 8 rows of every 32 (D = 128): eight lanes take four pieces of a row and the other four of the
+    // next one, so that their 16-byte reads and writes fall into eight different bank groups. A lane makes the factor of one of the warp's 32 rows, the
+    // others get it from there.
     const int tid = threadIdx.x - S::kConvWarp * 32;
     constexpr int kPieces = D / 16;               // of a row
     constexpr int kSteps = kBN * kPieces / 128;
@@ -518,30 +520,31 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           const uint8_t* src = raw + rs * S::kRawBytes;
           const uint8_t* sc = raw_scale + rs * kBN;
           uint8_t* dst = ring + slot * S::kSlotBytes;
-#pragma unroll 4
-          for (int i = 0; i < kSteps; ++i) {
-            int r, piece;
-            if (D == 128) {
-              const int pair = tid >> 3, half = (tid >> 2) & 1;             // rows 2 pair + half; i's lowest bit swaps the halves' pieces
-              r = (i >> 1) * 32 + pair * 2 + half;
-              piece = (tid & 3) + 4 * (half ^ (i & 1));
-            } else {
-              r = i * 32 + (tid >> 2);
-              piece = tid & 3;
+          const int cw = tid >> 5;
+          const int mine = (lane >> 3) * 32 + cw * 8 + (lane & 7);
+          Kv8Scale s = kv8_scale(mine < valid ? sc[mine] : 0);
+          const bool twice = __any_sync(0xffffffffu, s.twice);  // some value above 448 * 2^7
+          const auto convert = [&](auto both) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+              const int sub = lane >> 2;                   // row of the eight
+              const int r = (D == 128 ? i >> 1 : i) * 32 + cw * 8 + sub;
+              const int piece = D == 128 ? (lane & 3) + 4 * ((sub & 1) ^ (i & 1)) : lane & 3;
+              const int from = (D == 128 ? i >> 1 : i) * 8 + sub;
+              Kv8Scale f;
+              f.first = __shfl_sync(0xffffffffu, s.first, from);
+              f.second = decltype(both)::value ? __shfl_sync(0xffffffffu, s.second, from) : 0u;
+              f.twice = decltype(both)::value ? __shfl_sync(0xffffffffu, static_cast<int>(s.twice), from) != 0 : false;
+              const uint4 q = r < valid ? *reinterpret_cast<const uint4*>(src + r * D + piece * 16) : make_uint4(0u, 0u, 0u, 0u);
+              const uint2 a = kv8_decode4(q.x, f), b = kv8_decode4(q.y, f), c = kv8_decode4(q.z, f), d = kv8_decode4(q.w, f);
+              uint8_t* row = dst + (r >> 3) * kGroupBytes<D> + (piece >> 2) * 1024 + (r & 7) * 128;
+              const int ch = (piece & 3) * 2;
+              *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+              *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
             }
-            uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-            if (r < valid) {
-              const uint4 q = *reinterpret_cast<const uint4*>(src + r * D + piece * 16);
-              const Kv8Scale s = kv8_scale(sc[r]);
-              const uint2 a = kv8_decode4(q.x, s), b = kv8_decode4(q.y, s), c = kv8_decode4(q.z, s), d = kv8_decode4(q.w, s);
-              lo = make_uint4(a.x, a.y, b.x, b.y);
-              hi = make_uint4(c.x, c.y, d.x, d.y);
-            }
-            uint8_t* row = dst + (piece >> 2) * (kBN * 128) + r * 128;
-            const int ch = (piece & 3) * 2;
-            *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = lo;
-            *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = hi;
-          }
+          };
+          if (twice) convert(std::true_type{});
+          else convert(std::false_type{});
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -604,7 +607,6 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           const uint32_t tS = tmem + lanes + buf * 128 + (kFew ? quarter * 32 : 0);
           const int key0 = j * kBN + (kFew ? quarter * 32 : 0);
           const int see = pos - key0;                                         // columns up to this one
-          const bool masked = first_pos < key0 + (kFew ? 31 : kBN - 1);        // for some row
           // Rescales O and l where the maximum grew by more than 2^8; the products of the tile before must be complete then.
           const auto raise = [&](float mx) {
             mx *= p.scale_log2;
@@ -639,7 +641,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             l2.x *= alpha;
             l2.y *= alpha;
           };
-          const auto exponentials = [&](const uint32_t (&s)[32], int col, uint32_t dst) {  // 32 columns of P
+          const auto exponentials = [&](auto diag, const uint32_t (&s)[32], int col, uint32_t dst) {  // 32 columns of P
             const float base = m == -INFINITY ? 0.f : m;
             const float2 sc = make_float2(p.scale_log2, p.scale_log2), neg = make_float2(-base, -base);
             uint32_t pk[16];
@@ -647,7 +649,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             for (int i = 0; i < 32; i += 2) {
               const float2 z = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc, neg);
               float2 e = make_float2(exp2f(z.x), exp2f(z.y));
-              if (masked) {
+              if (decltype(diag)::value) {
                 if (col + i > see) e.x = 0.f;
                 if (col + i + 1 > see) e.y = 0.f;
               }
@@ -656,43 +658,44 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             }
             tmem_st_32x16(dst, pk);
           };
-          const auto top = [&](const uint32_t (&s)[32], int col, float (&mx)[4]) {
+          const auto top = [&](auto diag, const uint32_t (&s)[32], int col, float (&mx)[4]) {
+            const auto at = [&](int i) { return decltype(diag)::value && col + i > see ? -INFINITY : __uint_as_float(s[i]); };
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float v = __uint_as_float(s[i]);
-              if (masked && col + i > see) v = -INFINITY;
-              mx[i & 3] = fmaxf(mx[i & 3], v);
+            for (int i = 0; i < 32; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], at(i), at(i + 1));
+          };
+          const auto softmax = [&](auto diag) {  // diag: some row does not see the whole tile
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (kFew) {
+              uint32_t s[32];
+              tmem_ld_32x32(tS, s);
+              tc_wait_ld();
+              top(diag, s, 0, mx);
+              raise(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+              exponentials(diag, s, 0, tmem + lanes + kColP + buf * 64 + quarter * 16);
+            } else {
+              uint32_t s0[32], s1[32];
+              tmem_ld_32x32(tS, s0);
+              tmem_ld_32x32(tS + 32, s1);
+              tc_wait_ld();
+              top(diag, s0, 0, mx);
+              top(diag, s1, 32, mx);
+              tmem_ld_32x32(tS + 64, s0);
+              tmem_ld_32x32(tS + 96, s1);
+              tc_wait_ld();
+              top(diag, s0, 64, mx);
+              top(diag, s1, 96, mx);
+              raise(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+              exponentials(diag, s0, 64, tS + kColP + 32);
+              exponentials(diag, s1, 96, tS + kColP + 48);
+              tmem_ld_32x32(tS, s0);
+              tmem_ld_32x32(tS + 32, s1);
+              tc_wait_ld();
+              exponentials(diag, s0, 0, tS + kColP);
+              exponentials(diag, s1, 32, tS + kColP + 16);
             }
           };
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (kFew) {
-            uint32_t s[32];
-            tmem_ld_32x32(tS, s);
-            tc_wait_ld();
-            top(s, 0, mx);
-            raise(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-            exponentials(s, 0, tmem + lanes + kColP + buf * 64 + quarter * 16);
-          } else {
-            uint32_t s0[32], s1[32];
-            tmem_ld_32x32(tS, s0);
-            tmem_ld_32x32(tS + 32, s1);
-            tc_wait_ld();
-            top(s0, 0, mx);
-            top(s1, 32, mx);
-            tmem_ld_32x32(tS + 64, s0);
-            tmem_ld_32x32(tS + 96, s1);
-            tc_wait_ld();
-            top(s0, 64, mx);
-            top(s1, 96, mx);
-            raise(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-            exponentials(s0, 64, tS + kColP + 32);
-            exponentials(s1, 96, tS + kColP + 48);
-            tmem_ld_32x32(tS, s0);
-            tmem_ld_32x32(tS + 32, s1);
-            tc_wait_ld();
-            exponentials(s0, 0, tS + kColP);
-            exponentials(s1, 32, tS + kColP + 16);
-          }
+          if (first_pos < key0 + (kFew ? 31 : kBN - 1)) softmax(std::true_type{});
+          else softmax(std::false_type{});
           tc_wait_st();
         }
         tc_fence_before();
@@ -915,12 +918,16 @@ void launch(Params p, int num_sms, void* scratch, cudaStream_t s) {
   p.part_o = p.part_ml + static_cast<long long>(num_sms) * 2 * S::kRows * 2;
   const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.a.Hq), static_cast<uint64_t>(p.a.Tq)};
   const uint32_t box[3] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.tile_tokens)};
-  const CUtensorMap tq = make_tmap_3d(p.a.q, dims, D, p.a.ldq, box);
+  const uint64_t pitch[2] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.a.ldq)};
+  const CUtensorMap tq = make_tmap_nd<3>(p.a.q, dims, pitch, box);
   CUtensorMap tk = tq, tv = tq;  // 8 bits: not used
   if (!k8) {
-    const uint64_t rows = static_cast<uint64_t>(p.c.num_blocks) * p.c.Hkv * p.c.block_size;
-    tk = make_tmap_2d(p.c.k, D, rows, D, 64, p.c.block_size);
-    tv = make_tmap_2d(p.c.v, D, rows, D, 64, p.c.block_size);
+    // 64 columns, the 8 rows of a group, the columns' chunks, groups
+    const uint64_t kdims[4] = {64, 8, D / 64, static_cast<uint64_t>(p.c.num_blocks) * p.c.Hkv * p.c.block_size / 8};
+    const uint64_t kpitch[3] = {D, 64, 8 * D};
+    const uint32_t kbox[4] = {64, 8, D / 64, static_cast<uint32_t>(p.c.block_size / 8)};
+    tk = make_tmap_nd<4>(p.c.k, kdims, kpitch, kbox);
+    tv = make_tmap_nd<4>(p.c.v, kdims, kpitch, kbox);
   }
   auto kernel = paged_chunk_attn_kernel<D, k8, kFew>;
   AGRPO_SET_MAX_DYN_SMEM(kernel, S::kSmem, "paged_chunk_attn smem attr");
