@@ -15,7 +15,8 @@
 // share of the line. A CTA that gets a part of a unit leaves (O, m, l) in the workspace, and a second kernel adds the parts. So a single
 // long sequence fills the machine as a batch of ragged ones does, and nothing depends on lengths that the host would have to know.
 //
-// 8-bit cache: pages come as they are into a raw ring, four warps turn them into the bf16 tiles that the products read (kv8.cuh).
+// 8-bit cache: four warps, or four for K and four for V, bring the codes into shared memory, each thread what it will need, and turn them into the
+// bf16 tiles that the products read (kv8.cuh).
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -44,17 +45,24 @@ struct Shape {
   static constexpr int kRows = kFew ? 32 : 256;               // rows of a unit
   static constexpr int kSlotBytes = kBN * D * 2;              // a tile of K or V in bf16
   static constexpr int kQBytes = kTiles * 128 * D * 2;
-  static constexpr int kRawBytes = k8 ? kBN * D : 0;
-  static constexpr int kSlots = k8 ? 4 : (kFew ? 6 : 5);
-  static constexpr int kRaw = k8 ? (kFew ? 4 : 2) : 0;
+  static constexpr int kSlots = k8 ? (kFew ? 3 : 4) : (kFew ? 6 : 5);
+  static constexpr int kConvGroups = k8 ? (kFew ? 2 : 1) : 0;  // of four warps
+  // Item 2 i is K of the CTA's tile i, 2 i + 1 its V. Two groups fill slots of their own, one for K and two for V: in a ring for both, a group
+  // could not tell by a barrier's parity whether the other's tile before last has been read.
+  __device__ static __forceinline__ int slot(int item) { return kConvGroups == 2 ? ((item & 1) ? 1 + ((item >> 1) & 1) : 0) : item % kSlots; }
+  __device__ static __forceinline__ int round(int item) { return kConvGroups == 2 ? ((item & 1) ? item >> 2 : item >> 1) : item / kSlots; }
+  static constexpr int kDepth = kFew ? 3 : 2;                  // tiles of codes that a group has under way
+  static constexpr int kRaw = kConvGroups * kDepth;
   static constexpr int kSoftWarps = 4 * kTiles;
-  static constexpr int kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kConvWarp = kSoftWarps + 2;
-  static constexpr int kThreads = (kSoftWarps + 2 + (k8 ? 4 : 0)) * 32;
+  static constexpr int kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1;
+  // Four warpgroups where registers are dealt out anew (kShares): two warps of the third do nothing.
+  static constexpr bool kShares = k8 && !kFew;
+  static constexpr int kConvWarp = kSoftWarps + (kShares ? 4 : 2);
+  static constexpr int kThreads = (kConvWarp + 4 * kConvGroups) * 32;
   static constexpr int kRingOff = kQBytes;
   static constexpr int kRawOff = kRingOff + kSlots * kSlotBytes;
-  static constexpr int kScaleOff = kRawOff + kRaw * kRawBytes;
-  static constexpr int kMlOff = kScaleOff + kRaw * kBN;       // kFew: (m, l) of 4 warps x 32 rows
-  static constexpr int kBarOff = kMlOff + (kFew ? 1024 : 0);
+  static constexpr int kScaleOff = kRawOff + kRaw * kBN * D;
+  static constexpr int kBarOff = kScaleOff + kRaw * kBN;
   static constexpr int kBytes = kBarOff + 512;
   static constexpr int kSmem = kBytes + 1024;                 // room to align
   static_assert(kSmem <= kSmemLimit, "shared memory");
@@ -233,6 +241,24 @@ __device__ __forceinline__ void find_share(const Params& p, int* pref, int* at) 
   __syncthreads();
 }
 
+// 16 or 4 bytes into shared memory, zeros where `on` is false (nothing is read then).
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <bool kOn, int kLeft>
+__device__ __forceinline__ void give_registers() {
+  if (kOn) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeft));
+}
+
 template <int D, bool k8, bool kFew>
 __global__ void __launch_bounds__(Shape<D, k8, kFew>::kThreads, 1)
 paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -248,23 +274,19 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + S::kRingOff;
-  uint8_t* raw = smem + S::kRawOff;
-  uint8_t* raw_scale = smem + S::kScaleOff;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBarOff);
   uint64_t* full = bars;               // [kSlots]
   uint64_t* empty = bars + 6;          // [kSlots]
-  uint64_t* raw_full = bars + 12;      // [kRaw]
-  uint64_t* raw_empty = bars + 16;     // [kRaw]
-  uint64_t* q_full = bars + 20;
-  uint64_t* q_empty = bars + 21;
-  uint64_t* s_full = bars + 22;        // [2]
-  uint64_t* p_ready = bars + 24;       // [2]
-  uint64_t* o_done = bars + 26;        // [2]: after a piece's last product (of tile t); kFew: [0] after every one, [1] after the last. Softmax may be two
+  uint64_t* q_full = bars + 12;
+  uint64_t* q_empty = bars + 13;
+  uint64_t* s_full = bars + 14;        // [2]
+  uint64_t* p_ready = bars + 16;       // [2]
+  uint64_t* o_done = bars + 18;        // [2]: after a piece's last product (of tile t); kFew: [0] after every one, [1] after the last. Softmax may be two
                                        // products ahead at a piece's end, which one barrier for all of them could not tell from being done
-  uint64_t* o_free = bars + 28;        // [2]
-  uint64_t* soft = bars + 30;          // kFew: the softmax warps among themselves
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
-  int* at = reinterpret_cast<int*>(bars + 32);
+  uint64_t* o_free = bars + 20;        // [2]
+  uint64_t* soft = bars + 22;          // kFew: the softmax warps among themselves
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  int* at = reinterpret_cast<int*>(bars + 24);
   int* status = p.a.status;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -272,10 +294,6 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(full + i, k8 ? 4 : 1);
       mbar_init(empty + i, 1);
-    }
-    for (int i = 0; i < S::kRaw; ++i) {
-      mbar_init(raw_full + i, 1);
-      mbar_init(raw_empty + i, 4);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, kFew ? 5 : 1);
@@ -302,55 +320,45 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   Walk w;
   w.start(p, at);
 
+  // kShares: 128 x (168 + 168 + 72 + 104) registers = 512 x 128
   if (warp == S::kLoadWarp) {
+    give_registers<S::kShares, 72>();
     // ---------------------------------------------------------------- copies
-    // Item i of the ring is K (even) or V (odd) of the CTA's tile i / 2. The first tile of a piece goes ahead of its Q, which has to wait for
-    // the last products with the one before.
+    // The first tile of a piece goes ahead of its Q, which has to wait for the last products with the one before. (8 bits: Q alone comes from here.)
     int item = 0, n_q = 0;
     bool ok = true;
-    constexpr int kStages = k8 ? (S::kRaw > 0 ? S::kRaw : 1) : S::kSlots;
     for (; w.more() && ok; w.next(p)) {
       const int* table = p.a.block_tables + w.b * p.a.table_pitch;
       const int keys = unit_keys(p, w.s, w.qb);
       const int bs = p.c.block_size;
-      const int page_of_lane = k8 ? lane & 15 : lane;
       const auto page_id = [&](int j) {
-        const int key = j * kBN + page_of_lane * bs;
-        int id = page_of_lane * bs < kBN && key < keys ? table[key / bs] : 0;
+        const int key = j * kBN + lane * bs;
+        int id = lane * bs < kBN && key < keys ? table[key / bs] : 0;
         if (id < 0 || id >= p.c.num_blocks) {
           report_status(status, kStatusBadIndex);
           id = 0;
         }
         return id;
       };
-      int id = page_id(w.j0);
-      for (int j = w.j0; j < w.j1 && ok; ++j) {
-        const int pages = (min(kBN, keys - j * kBN) + bs - 1) / bs;  // none in a unit without keys
-        const long long row = (static_cast<long long>(id) * p.c.Hkv + w.kvh) * bs;
-        if (j + 1 < w.j1) id = page_id(j + 1);
+      int id = k8 ? 0 : page_id(w.j0);
+      for (int j = w.j0; j < (k8 ? w.j0 + 1 : w.j1) && ok; ++j) {
+        if (!k8) {
+          const int pages = (min(kBN, keys - j * kBN) + bs - 1) / bs;  // none in a unit without keys
+          const long long row = (static_cast<long long>(id) * p.c.Hkv + w.kvh) * bs;
+          if (j + 1 < w.j1) id = page_id(j + 1);
 #pragma unroll 1
-        for (int v = 0; v < 2 && ok; ++v, ++item) {
-          const int slot = item % kStages;
-          uint64_t* const e = (k8 ? raw_empty : empty) + slot;
-          uint64_t* const f = (k8 ? raw_full : full) + slot;
-          if (item >= kStages && !mbar_wait(e, (item / kStages - 1) & 1)) {
-            report_status(status, kStatusWaitEmptyTimeout);
-            ok = false;
-            break;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_expect_tx(f, pages * bs * (k8 ? D + 1 : D * 2));
-          __syncwarp();
-          if (page_of_lane < pages) {
-            if (k8) {
-              if (lane < 16) {
-                bulk_load_g2s(raw + slot * S::kRawBytes + page_of_lane * bs * D, static_cast<const uint8_t*>(v ? p.c.v : p.c.k) + row * D, bs * D, f);
-              } else {
-                bulk_load_g2s(raw_scale + slot * kBN + page_of_lane * bs, (v ? p.c.v_scale : p.c.k_scale) + row, bs, f);
-              }
-            } else {
-              tma_load_4d(ring + slot * S::kSlotBytes + page_of_lane * (bs / 8) * kGroupBytes<D>, v ? &tmV : &tmK, f, 0, 0, 0, static_cast<int>(row >> 3));
+          for (int v = 0; v < 2 && ok; ++v, ++item) {
+            const int slot = S::slot(item), round = S::round(item);
+            if (round > 0 && !mbar_wait(empty + slot, (round - 1) & 1)) {
+              report_status(status, kStatusWaitEmptyTimeout);
+              ok = false;
+              break;
             }
+            __syncwarp();
+            if (lane == 0) mbar_expect_tx(full + slot, pages * bs * D * 2);
+            __syncwarp();
+            if (lane < pages)
+              tma_load_4d(ring + slot * S::kSlotBytes + lane * (bs / 8) * kGroupBytes<D>, v ? &tmV : &tmK, full + slot, 0, 0, 0, static_cast<int>(row >> 3));
           }
         }
         if (j == w.j0 && ok) {
@@ -376,6 +384,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
     }
   } else if (warp == S::kMmaWarp) {
+    give_registers<S::kShares, 72>();
     // ---------------------------------------------------------------- products
     const uint32_t aQ = smem_u32(smem), aRing = smem_u32(ring);
     int tile = 0, n_q = 0;          // tiles and pieces so far
@@ -389,11 +398,11 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       return ok;
     };
-    const auto slot_wait = [&](int item) { return wait(full + item % S::kSlots, (item / S::kSlots) & 1, kStatusWaitFullTimeout); };
+    const auto slot_wait = [&](int item) { return wait(full + S::slot(item), S::round(item) & 1, kStatusWaitFullTimeout); };
     const auto scores = [&](int t, int item, uint32_t col) {  // S = Q_t K^T
       if (elect_one()) {
-        const uint32_t q = aQ + t * (128 * D * 2), k = aRing + (item % S::kSlots) * S::kSlotBytes;
-#pragma unroll
+        const uint32_t q = aQ + t * (128 * D * 2), k = aRing + S::slot(item) * S::kSlotBytes;
+#pragma unroll 1  // unrolled, the descriptors would stay in registers from one tile to the next
         for (int i = 0; i < D / 16; ++i) {
           tc_mma_f16(tmem + col, umma_smem_desc(q + (i / 4) * (128 * 128) + (i % 4) * 32, 16, 1024),
                      umma_smem_desc(k + (i / 4) * 1024 + (i % 4) * 32, 16, kGroupBytes<D>), kIdescS, i > 0 ? 1u : 0u);
@@ -404,8 +413,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     };
     const auto values = [&](int item, uint32_t col_p, uint32_t col_o, bool first) {  // O (+)= P V
       if (elect_one()) {
-        const uint32_t v = aRing + (item % S::kSlots) * S::kSlotBytes;
-#pragma unroll
+        const uint32_t v = aRing + S::slot(item) * S::kSlotBytes;
+#pragma unroll 1
         for (int i = 0; i < kBN / 16; ++i)
           tc_mma_f16_ts(tmem + col_o, tmem + col_p + i * 8, umma_smem_desc(v + i * 2 * kGroupBytes<D>, 1024, kGroupBytes<D>), kIdescO, (!first || i > 0) ? 1u : 0u);
       }
@@ -418,7 +427,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     // Rows of V behind the last visible key: whatever the page held before, 0 * NaN would reach every row. (The converting warps do it for 8 bits.)
     const auto clear_tail = [&](int item, int valid) {
       if (k8 || valid >= kBN) return;
-      uint8_t* v = ring + (item % S::kSlots) * S::kSlotBytes;
+      uint8_t* v = ring + S::slot(item) * S::kSlotBytes;
       for (int i = max(valid, 0) * 8 + lane; i < kBN * 8; i += 32) {  // row i / 8, bytes (i % 8) * 16 of its atoms
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(v + (i >> 6) * kGroupBytes<D> + c * 1024 + (i & 63) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -433,14 +442,14 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         if (!slot_wait(2 * tile)) break;
         tc_fence_after();
         scores(0, 2 * tile, (tile & 1) * 128);
-        commit(empty + (2 * tile) % S::kSlots);
+        commit(empty + S::slot(2 * tile));
         for (int j = w.j0; j < w.j1; ++j, ++tile) {
           if (j + 1 < w.j1) {
             const int item = 2 * tile + 2;
             if (!slot_wait(item)) break;
             tc_fence_after();
             scores(0, item, ((tile + 1) & 1) * 128);
-            commit(empty + item % S::kSlots);
+            commit(empty + S::slot(item));
           }
           if (j + 1 >= w.j1) commit(q_empty);
           if (j == w.j0 && n_o[0] > 0 && !wait(o_free, (n_o[0] - 1) & 1, kStatusWaitTmemEmptyTimeout)) break;
@@ -451,7 +460,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           values(2 * tile + 1, kColP + (tile & 1) * 64, kColO, j == w.j0);
           commit(o_done);
           if (j + 1 >= w.j1) commit(o_done + 1);
-          commit(empty + (2 * tile + 1) % S::kSlots);
+          commit(empty + S::slot(2 * tile + 1));
         }
         ++n_o[0];
       } else {
@@ -460,7 +469,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         tc_fence_after();
         for (int t = 0; t < 2; ++t)
           if (w.j0 < end[t]) scores(t, 2 * tile, t * 128);
-        commit(empty + (2 * tile) % S::kSlots);
+        commit(empty + S::slot(2 * tile));
         for (int j = w.j0; j < w.j1 && ok; ++j, ++tile) {
           if (j + 1 >= w.j1) commit(q_empty);
           if (!slot_wait(2 * tile + 1)) break;
@@ -482,79 +491,124 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
               scores(t, 2 * tile + 2, t * 128);
             }
           }
-          commit(empty + (2 * tile + 1) % S::kSlots);
+          commit(empty + S::slot(2 * tile + 1));
           if (more) {
             slot_wait(2 * tile + 2);  // where no tile of Q takes part any more, it still counts as read
-            commit(empty + (2 * tile + 2) % S::kSlots);
+            commit(empty + S::slot(2 * tile + 2));
           }
         }
       }
     }
   } else if (k8 && warp >= S::kConvWarp) {
+    give_registers<S::kShares, 104>();
     // ---------------------------------------------------------------- 8 bits to bf16
-    // 16 codes a thread and step. A warp has 8 rows of every 32 (D = 128): eight lanes take four pieces of a row and the other four of the
-    // next one, so that their 16-byte reads and writes fall into eight different bank groups. A lane makes the factor of one of the warp's 32 rows, the
-    // others get it from there.
-    const int tid = threadIdx.x - S::kConvWarp * 32;
-    constexpr int kPieces = D / 16;               // of a row
-    constexpr int kSteps = kBN * kPieces / 128;
-    int item = 0;
+    // 16 codes a thread and step. A warp has 8 rows of every 32 (two steps for them if D = 128): eight lanes take four pieces of a row and the other
+    // four of the next one, so that their 16-byte writes fall into eight different bank groups. A thread copies the pieces that it will turn into bf16
+    // itself, so nobody waits for anybody else's copies, kDepth tiles ahead. (Bulk copies of pages of 16 tokens, 2 KB, took 54 cycles each to issue.)
+    const int group = (warp - S::kConvWarp) >> 2, cw = (warp - S::kConvWarp) & 3, tid = cw * 32 + lane;
+    constexpr int kGroups = S::kConvGroups > 0 ? S::kConvGroups : 1;
+    constexpr int kPerRows = D / 64;             // steps for the same rows
+    uint8_t* raw = smem + S::kRawOff + group * S::kDepth * (kBN * D) + tid * 16;
+    uint8_t* raw_scale = smem + S::kScaleOff + group * S::kDepth * kBN + cw * 32;
+    const int sub = lane >> 2;                   // row of the eight
+    Walk a = w;                                  // the copies' walk
+    int a_j = a.j0, a_v = group, n_copy = 0, page = 0;
+    // Blocks of the table that hold this warp's rows of the tile: lane i < 4 those from row 32 i + 8 cw on.
+    const auto pages = [&] {
+      if (!a.more()) return;
+      const int key = a_j * kBN + (lane & 3) * 32 + cw * 8;
+      page = key < unit_keys(p, a.s, a.qb) ? p.a.block_tables[a.b * p.a.table_pitch + key / p.c.block_size] : 0;
+    };
+    const auto copy = [&] {
+      if (a.more()) {
+        if (page < 0 || page >= p.c.num_blocks) {
+          report_status(status, kStatusBadIndex);
+          page = 0;
+        }
+        const int slot = n_copy % S::kDepth, bs = p.c.block_size;
+        const int valid = unit_keys(p, a.s, a.qb) - a_j * kBN;
+        const auto* codes = static_cast<const uint8_t*>(a_v ? p.c.v : p.c.k);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = q * 32 + cw * 8 + sub;
+          const long long row = (static_cast<long long>(__shfl_sync(0xffffffffu, page, q)) * p.c.Hkv + a.kvh) * bs + ((a_j * kBN + r) & (bs - 1));
+#pragma unroll
+          for (int h = 0; h < kPerRows; ++h) {
+            const int piece = D == 128 ? (lane & 3) + 4 * ((sub & 1) ^ h) : lane & 3;
+            cp_async_16(raw + slot * (kBN * D) + (q * kPerRows + h) * 2048, codes + row * D + piece * 16, r < valid);
+          }
+        }
+        // the factors' bytes: four rows a lane
+        const int pq = __shfl_sync(0xffffffffu, page, lane >> 1 & 3), r = (lane >> 1 & 3) * 32 + cw * 8 + (lane & 1) * 4;
+        if (lane < 8) {
+          const long long row = (static_cast<long long>(pq) * p.c.Hkv + a.kvh) * bs + ((a_j * kBN + r) & (bs - 1));
+          cp_async_4(raw_scale + slot * kBN + lane * 4, (a_v ? p.c.v_scale : p.c.k_scale) + row, r < valid);
+        }
+        ++n_copy;
+        a_v += kGroups;
+        if (a_v > 1) {
+          a_v = group;
+          if (++a_j == a.j1) {
+            a.next(p);
+            a_j = a.j0;
+          }
+          pages();
+        }
+      }
+      cp_async_commit();  // also where nothing is left, so that the waits below name the same tile
+    };
+    pages();
+#pragma unroll 1
+    for (int i = 0; i < S::kDepth; ++i) copy();
+    int item = group, n = 0;
     bool ok = true;
     for (; w.more() && ok; w.next(p)) {
-      const int keys = unit_keys(p, w.s, w.qb);
       for (int j = w.j0; j < w.j1 && ok; ++j) {
-        const int valid = min(kBN, keys - j * kBN);
-        for (int v = 0; v < 2 && ok; ++v, ++item) {
-          constexpr int kRaw = S::kRaw > 0 ? S::kRaw : 1;  // without 8 bits nothing comes here
-          const int rs = item % kRaw, slot = item % S::kSlots;
-          if (!mbar_wait(raw_full + rs, (item / kRaw) & 1)) {
-            report_status(status, kStatusWaitFullTimeout);
-            ok = false;
-            break;
-          }
-          if (item >= S::kSlots && !mbar_wait(empty + slot, (item / S::kSlots - 1) & 1)) {
+        for (int v = group; v < 2 && ok; v += kGroups, item += kGroups, ++n) {
+          const int slot = S::slot(item), round = S::round(item), mine = n % S::kDepth;
+          cp_async_wait<S::kDepth - 1>();
+          __syncwarp();
+          // of row 32 (lane / 8) + 8 cw + lane % 8. Behind the last key the codes are zero, and the factor has to be a number
+          const int left = unit_keys(p, w.s, w.qb) - j * kBN - cw * 8;
+          const Kv8Scale s = kv8_scale((lane >> 3) * 32 + (lane & 7) < left ? raw_scale[mine * kBN + lane] : 0);
+          const bool twice = __any_sync(0xffffffffu, s.twice);         // some value above 448 * 2^7
+          if (round > 0 && !mbar_wait(empty + slot, (round - 1) & 1)) {
             report_status(status, kStatusWaitEmptyTimeout);
             ok = false;
             break;
           }
-          const uint8_t* src = raw + rs * S::kRawBytes;
-          const uint8_t* sc = raw_scale + rs * kBN;
-          uint8_t* dst = ring + slot * S::kSlotBytes;
-          const int cw = tid >> 5;
-          const int mine = (lane >> 3) * 32 + cw * 8 + (lane & 7);
-          Kv8Scale s = kv8_scale(mine < valid ? sc[mine] : 0);
-          const bool twice = __any_sync(0xffffffffu, s.twice);  // some value above 448 * 2^7
+          const uint8_t* src = raw + mine * (kBN * D);
+          uint8_t* dst = ring + slot * S::kSlotBytes + cw * kGroupBytes<D> + sub * 128;
           const auto convert = [&](auto both) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-              const int sub = lane >> 2;                   // row of the eight
-              const int r = (D == 128 ? i >> 1 : i) * 32 + cw * 8 + sub;
-              const int piece = D == 128 ? (lane & 3) + 4 * ((sub & 1) ^ (i & 1)) : lane & 3;
-              const int from = (D == 128 ? i >> 1 : i) * 8 + sub;
+            for (int q = 0; q < 4; ++q) {
               Kv8Scale f;
-              f.first = __shfl_sync(0xffffffffu, s.first, from);
-              f.second = decltype(both)::value ? __shfl_sync(0xffffffffu, s.second, from) : 0u;
-              f.twice = decltype(both)::value ? __shfl_sync(0xffffffffu, static_cast<int>(s.twice), from) != 0 : false;
-              const uint4 q = r < valid ? *reinterpret_cast<const uint4*>(src + r * D + piece * 16) : make_uint4(0u, 0u, 0u, 0u);
-              const uint2 a = kv8_decode4(q.x, f), b = kv8_decode4(q.y, f), c = kv8_decode4(q.z, f), d = kv8_decode4(q.w, f);
-              uint8_t* row = dst + (r >> 3) * kGroupBytes<D> + (piece >> 2) * 1024 + (r & 7) * 128;
-              const int ch = (piece & 3) * 2;
-              *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
-              *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
+              f.first = __shfl_sync(0xffffffffu, s.first, q * 8 + sub);
+              f.second = decltype(both)::value ? __shfl_sync(0xffffffffu, s.second, q * 8 + sub) : 0u;
+              f.twice = decltype(both)::value ? __shfl_sync(0xffffffffu, static_cast<int>(s.twice), q * 8 + sub) != 0 : false;
+#pragma unroll
+              for (int h = 0; h < kPerRows; ++h) {
+                const uint4 x = *reinterpret_cast<const uint4*>(src + (q * kPerRows + h) * 2048);
+                const uint2 e = kv8_decode4(x.x, f), g = kv8_decode4(x.y, f), y = kv8_decode4(x.z, f), z = kv8_decode4(x.w, f);
+                uint8_t* row = dst + q * 4 * kGroupBytes<D> + (D == 128 ? ((sub & 1) ^ h) * 1024 : 0);
+                const int ch = (lane & 3) * 2;
+                *reinterpret_cast<uint4*>(row + ((ch ^ sub) << 4)) = make_uint4(e.x, e.y, g.x, g.y);
+                *reinterpret_cast<uint4*>(row + (((ch + 1) ^ sub) << 4)) = make_uint4(y.x, y.y, z.x, z.y);
+              }
             }
           };
           if (twice) convert(std::true_type{});
           else convert(std::false_type{});
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(raw_empty + rs);
-            mbar_arrive(full + slot);
-          }
+          if (lane == 0) mbar_arrive(full + slot);
+          copy();
         }
       }
     }
+    cp_async_wait<0>();
   } else if (warp < S::kSoftWarps) {
+    if (S::kShares) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ---------------------------------------------------------------- softmax, results
     const int t = kFew ? 0 : warp >> 2, quarter = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -717,7 +771,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       auto* out = static_cast<__nv_bfloat16*>(p.a.out);
       if (kFew) {
         // the quarters of O: weights by maximum, added through the shared memory of Q, 64 columns at a time
-        float2* ml = reinterpret_cast<float2*>(smem + S::kMlOff);
+        float2* ml = reinterpret_cast<float2*>(smem);
         ml[quarter * 32 + lane] = make_float2(m, l);
         soft_sync();
         float M = -INFINITY, L = 0.f;
@@ -731,35 +785,37 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           const float2 x = ml[q * 32 + lane];
           if (x.y != 0.f) L += x.y * exp2f(x.x - M);
         }
+        soft_sync();
         const float weight = l != 0.f ? exp2f(m - M) : 0.f;
         const float scale = !whole ? 1.f : (L != 0.f ? 1.f / L : 0.f);
-        uint8_t* buf = smem;  // [4][32 rows][16 chunks of 16 bytes], chunk c of a row at c ^ (row & 15)
+        constexpr int kPass = D / 2, kVec = kPass / 4;  // columns at a time: what fits into Q's memory
+        static_assert(4 * 32 * kPass * 4 <= S::kQBytes, "the quarters of O go through the memory of Q");
+        uint8_t* buf = smem;  // [4][32 rows][kVec chunks of 16 bytes], chunk c of a row at c ^ (row & (kVec - 1))
+        const auto at_row = [&](int q, int row, int ch) { return reinterpret_cast<float4*>(buf + ((q * 32 + row) * kVec + (ch ^ (row & (kVec - 1)))) * 16); };
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 64) {
+        for (int c0 = 0; c0 < D; c0 += kPass) {
 #pragma unroll 1
-          for (int h = 0; h < 64; h += 32) {
+          for (int h = 0; h < kPass; h += 32) {
             uint32_t o[32];
             tmem_ld_32x32(tO + c0 + h, o);
             tc_wait_ld();
             if (lane < rows) {
               const float f = weight * scale;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int ch = h / 4 + i;
-                const float4 x = weight == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                               : make_float4(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f, __uint_as_float(o[4 * i + 2]) * f,
-                                                             __uint_as_float(o[4 * i + 3]) * f);
-                *reinterpret_cast<float4*>(buf + (quarter * 32 + lane) * 256 + ((ch ^ (lane & 15)) << 4)) = x;
-              }
+              for (int i = 0; i < 8; ++i)
+                *at_row(quarter, lane, h / 4 + i) =
+                    weight == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                  : make_float4(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f, __uint_as_float(o[4 * i + 2]) * f,
+                                                __uint_as_float(o[4 * i + 3]) * f);
             }
           }
           soft_sync();
-          for (int i = threadIdx.x; i < rows * 16; i += 128) {
-            const int row = i >> 4, ch = i & 15;
+          for (int i = threadIdx.x; i < rows * kVec; i += 128) {
+            const int row = i / kVec, ch = i % kVec;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const float4 y = *reinterpret_cast<const float4*>(buf + (q * 32 + row) * 256 + ((ch ^ (row & 15)) << 4));
+              const float4 y = *at_row(q, row, ch);
               x.x += y.x;
               x.y += y.y;
               x.z += y.z;
@@ -832,6 +888,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
     }
   }
+
+  if (S::kShares && warp > S::kLoadWarp && warp < S::kConvWarp) give_registers<S::kShares, 72>();
 
   tc_fence_before();
   __syncthreads();
