@@ -1,0 +1,302 @@
+// What the two kernels of paged_chunk_attn share: how a call's work lies in a line, how workers take equal shares of it, and how the parts of a unit
+// that several of them worked on are added.
+//
+// A unit is the rows of some tokens of a sequence under one kv head (row = token * G + query head of the group). All units lie in a line, sequence
+// by sequence, kv head by kv head; a unit is as long as it has tiles of kKeys keys to look at. W workers (CTAs or warps; as many as there are, or as many as find
+// work for their while) take the tiles [T w / W, T (w + 1) / W) of the T tiles. So one long sequence fills the machine as a batch of ragged ones does, shares differ
+// by one tile at most, and nothing depends on a length that the host would have to know. A worker that has a part of a unit leaves (O, m, l) in the workspace:
+// only its first and its last piece can be parts. Parts are added in the order of the keys, so the same call gives the same bits.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "../common/ptx.cuh"
+#include "../launchers.h"
+#include "../launchers_cache.h"
+
+namespace agrpo {
+
+namespace {
+
+struct LineParams {
+  ChunkAttnArgs a;
+  PagedCache c;
+  int G, tokens;      // query heads a kv head; tokens a unit
+  int tile_tokens;    // tokens a tile of rows
+  int rows;           // rows that a part has room for
+  float scale_log2;
+  int4* desc;         // [CTAs]: the unit that starts in the CTA and ends in a later one {first row, tokens, kv head, last CTA}
+  float* part_ml;     // [CTAs, 2, rows, 2]: parts, [0] of a unit that an earlier CTA starts, [1] of one that starts here
+  float* part_o;      // [CTAs, 2, rows, D]
+  float* warp_ml;     // the same of warps, where those are the workers
+  float* warp_o;
+};
+
+struct Seq {
+  int row0, n, len;
+  bool bad;
+};
+__device__ __forceinline__ Seq load_seq(const LineParams& p, int b) {
+  Seq s;
+  s.row0 = p.a.q_starts[b];
+  const int end = p.a.q_starts[b + 1];
+  s.len = max(p.a.seq_lens[b], 0);
+  s.bad = s.row0 < 0 || end < s.row0 || end > p.a.Tq;
+  s.n = s.bad ? 0 : end - s.row0;
+  if (s.len > p.a.max_blocks * p.c.block_size) {
+    s.bad = true;
+    s.len = 0;
+  }
+  return s;
+}
+// Keys that the last row of unit qb sees, and tiles of them. A unit without keys still has a tile: its rows are zeros to be written.
+__device__ __forceinline__ int unit_keys(const LineParams& p, const Seq& s, int qb) { return max(s.len - s.n + min(s.n, (qb + 1) * p.tokens), 0); }
+template <int kKeys>
+__device__ __forceinline__ int unit_tiles(const LineParams& p, const Seq& s, int qb) {
+  return max(1, (unit_keys(p, s, qb) + kKeys - 1) / kKeys);
+}
+__device__ __forceinline__ int num_units(const LineParams& p, const Seq& s) { return (s.n + p.tokens - 1) / p.tokens; }
+
+// Where a worker's share begins.
+struct Share {
+  int b, kvh, qb, j;   // sequence, kv head, unit, tile
+  int tiles, before;   // of the share, ahead of it
+  int total, workers;  // of the line; that have a share
+};
+
+// A worker's walk along its share: one piece (tiles [j0, j1) of a unit) after the other.
+template <int kKeys>
+struct Walk {
+  Seq s;
+  int b, kvh, qb, j0, j1, nk, left;
+
+  __device__ __forceinline__ void start(const LineParams& p, const Share& at) {
+    b = at.b;
+    kvh = at.kvh;
+    qb = at.qb;
+    j0 = at.j;
+    left = at.tiles;
+    if (left > 0) {
+      s = load_seq(p, b);
+      clip(p);
+    }
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void clip(const LineParams& p) {
+    nk = unit_tiles<kKeys>(p, s, qb);
+    j1 = min(nk, j0 + left);
+  }
+  __device__ __forceinline__ void next(const LineParams& p) {
+    left -= j1 - j0;
+    if (left <= 0) return;
+    j0 = 0;
+    if (++qb == num_units(p, s)) {
+      qb = 0;
+      if (++kvh == p.c.Hkv) {
+        kvh = 0;
+        do s = load_seq(p, ++b);
+        while (s.n == 0);
+      }
+    }
+    clip(p);
+  }
+  __device__ __forceinline__ int tokens(const LineParams& p) const { return min(p.tokens, s.n - qb * p.tokens); }
+  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nk; }
+  __device__ __forceinline__ int part(int worker) const { return worker * 2 + (j0 == 0 ? 1 : 0); }
+  // Tiles of this piece that tile t of the rows takes part in: [j0, end).
+  __device__ __forceinline__ int end_of(const LineParams& p, int t) const {
+    const int tok = min(p.tile_tokens * (t + 1), tokens(p));
+    if (tok <= p.tile_tokens * t) return j0;
+    const int keys = s.len - s.n + qb * p.tokens + tok;
+    return max(j0, min(j1, (keys + kKeys - 1) / kKeys));
+  }
+  // The worker that has the unit's last tile, `flat` tiles of the line being ahead of this piece.
+  __device__ __forceinline__ int last_worker(const Share& at, int flat) const {
+    const long long end = flat - j0 + nk;
+    return static_cast<int>((end * at.workers + at.total - 1) / at.total) - 1;
+  }
+};
+
+// The line up to each sequence's end, into `line` (B ints of shared memory). All threads of the CTA; reports sequences that cannot be.
+template <int kThreads, int kKeys>
+__device__ __forceinline__ void measure_line(const LineParams& p, int* line) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < p.a.B; base += kThreads) {
+    const int b = base + threadIdx.x;
+    Seq s = {0, 0, 0, false};
+    if (b < p.a.B) s = load_seq(p, b);
+    if (s.bad && blockIdx.x == 0) report_status(p.a.status, kStatusBadIndex);
+    const int units = num_units(p, s);
+    int mine = 0;
+    if (units <= 8)
+      for (int q = 0; q < units; ++q) mine += unit_tiles<kKeys>(p, s, q);
+    for (unsigned big = __ballot_sync(0xffffffffu, units > 8); big != 0; big &= big - 1) {  // the warp together
+      const int src = __ffs(big) - 1;
+      Seq o = s;
+      o.n = __shfl_sync(0xffffffffu, s.n, src);
+      o.len = __shfl_sync(0xffffffffu, s.len, src);
+      const int total = num_units(p, o);
+      int sum = 0;
+      for (int q = lane; q < total; q += 32) sum += unit_tiles<kKeys>(p, o, q);
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      if (lane == src) mine = sum;
+    }
+    if (b < p.a.B) line[b] = mine * p.c.Hkv;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int run = 0;
+    for (int base = 0; base < p.a.B; base += 32) {
+      int v = base + lane < p.a.B ? line[base + lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      v += run;
+      run = __shfl_sync(0xffffffffu, v, 31);
+      if (base + lane < p.a.B) line[base + lane] = v;
+    }
+  }
+  __syncthreads();
+}
+
+// A worker's share, of kLeast tiles at least if there are so many. One warp, all lanes with the same result.
+template <int kKeys, int kLeast>
+__device__ __forceinline__ Share find_share(const LineParams& p, const int* line, int worker, int workers) {
+  const int lane = threadIdx.x & 31;
+  Share at = {0, 0, 0, 0, 0, 0, line[p.a.B - 1], 0};
+  at.workers = min(workers, (at.total + kLeast - 1) / kLeast);
+  if (worker >= at.workers) return at;
+  at.before = static_cast<int>(static_cast<long long>(at.total) * worker / at.workers);
+  at.tiles = static_cast<int>(static_cast<long long>(at.total) * (worker + 1) / at.workers) - at.before;
+  int hi = p.a.B - 1;
+  while (at.b < hi) {
+    const int mid = (at.b + hi) / 2;
+    if (line[mid] > at.before) hi = mid;
+    else at.b = mid + 1;
+  }
+  const int ahead = at.b > 0 ? line[at.b - 1] : 0;
+  const int per = (line[at.b] - ahead) / p.c.Hkv;
+  int r = at.before - ahead;
+  at.kvh = r / per;
+  r -= at.kvh * per;
+  const Seq s = load_seq(p, at.b);
+  for (int q0 = 0; q0 < num_units(p, s); q0 += 32) {
+    const int q = q0 + lane;
+    const int nk = q < num_units(p, s) ? unit_tiles<kKeys>(p, s, q) : 0;
+    int inc = nk;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, inc > r);
+    if (past != 0) {
+      const int src = __ffs(past) - 1;
+      at.qb = q0 + src;
+      at.j = r - __shfl_sync(0xffffffffu, inc - nk, src);
+      break;
+    }
+    r -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return at;
+}
+
+// One row's share of a unit: adds the parts first .. last (the first in place `head` of its pair, the others in 0). A warp; lane i gets dims i D / 32 and on, and
+// every lane the row's maximum and sum.
+template <int D>
+__device__ __forceinline__ void add_parts(const float* part_ml, const float* part_o, int rows, int row, int first, int last, int head, float (&o)[D / 32], float& M,
+                                          float& L) {
+  constexpr int kPer = D / 32;
+  const int lane = threadIdx.x & 31;
+  M = -INFINITY;
+  L = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+  for (int k0 = first; k0 <= last; k0 += 32) {
+    const int k = min(k0 + lane, last);
+    float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + ((static_cast<long long>(k) * 2 + (k == first ? head : 0)) * rows + row) * 2));
+    if (k0 + lane > last) ml.y = 0.f;
+    float mx = ml.y != 0.f ? ml.x : -INFINITY;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    const float Mn = fmaxf(M, mx);
+    const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
+    const float wgt = ml.y != 0.f ? exp2f(ml.x - Mn) : 0.f;
+    float ls = ml.y * wgt;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, off);
+    L = L * keep + ls;
+    M = Mn;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] *= keep;
+    // eight parts at a time, their loads without a condition between them
+    for (int i0 = 0; i0 < min(32, last - k0 + 1); i0 += 8) {
+      float x[8][kPer];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int part = min(k0 + i0 + i, last);
+        const float* src = part_o + ((static_cast<long long>(part) * 2 + (part == first ? head : 0)) * rows + row) * D + lane * kPer;
+        if (kPer == 4) *reinterpret_cast<float4*>(x[i]) = __ldcg(reinterpret_cast<const float4*>(src));
+        else *reinterpret_cast<float2*>(x[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, wgt, i0 + i);
+        if (wi == 0.f) continue;  // no keys: what lies there means nothing
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) o[d] += x[i][d] * wi;
+      }
+    }
+  }
+}
+// The finished row of a unit into the output.
+template <int D>
+__device__ __forceinline__ void store_row(const LineParams& p, int row0, int kvh, int r, const float (&o)[D / 32], float L) {
+  constexpr int kPer = D / 32;
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  const int tk = r / p.G, hd = r - tk * p.G;
+  auto* dst = static_cast<__nv_bfloat16*>(p.a.out) + static_cast<long long>(row0 + tk) * p.a.ldo + static_cast<long long>(kvh * p.G + hd) * D +
+              (threadIdx.x & 31) * kPer;
+  uint32_t y[kPer / 2];
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) y[i] = pack_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
+  if (kPer == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[kPer / 2 - 1]);
+  else *reinterpret_cast<uint32_t*>(dst) = y[0];
+}
+
+// Adds the parts of the units that several CTAs had. A warp a row, 8 rows of one unit a block.
+template <int D>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const LineParams p) {
+  pdl_wait();
+  pdl_launch();
+  const int c = blockIdx.x;
+  const int4 u = p.desc[c];
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= u.y * p.G) return;
+  const int tile = r / p.G / p.tile_tokens;  // a tile's rows start on 128
+  float o[D / 32], M, L;
+  add_parts<D>(p.part_ml, p.part_o, p.rows, r + tile * (128 - p.tile_tokens * p.G), c, u.w, 1, o, M, L);
+  store_row<D>(p, u.x, u.z, r, o, L);
+}
+
+// Workspace of a launch: what LineParams points to.
+inline long long line_scratch(int ctas, int warps, int rows, int D) { return ctas * 16ll + static_cast<long long>(ctas) * (1 + warps) * 2 * rows * (2 + D) * 4; }
+inline void place_scratch(LineParams& p, void* scratch, int ctas, int warps, int rows, int D) {
+  p.rows = rows;
+  p.desc = static_cast<int4*>(scratch);
+  p.part_ml = reinterpret_cast<float*>(p.desc + ctas);
+  p.part_o = p.part_ml + static_cast<long long>(ctas) * 2 * rows * 2;
+  p.warp_ml = p.part_o + static_cast<long long>(ctas) * 2 * rows * D;
+  p.warp_o = p.warp_ml + static_cast<long long>(ctas) * warps * 2 * rows * 2;
+}
+template <int D>
+inline void launch_combine(const LineParams& p, int ctas, cudaStream_t s) {
+  auto combine = paged_combine_kernel<D>;
+  AGRPO_PREFER_SMEM(combine);
+  launch_kernel(combine, dim3(ctas, (p.rows + 7) / 8), dim3(256), 0, s, "paged_combine", p);
+}
+
+}  // namespace
+
+}  // namespace agrpo
