@@ -2,7 +2,7 @@
 //
 // Sequence b has n = q_starts[b + 1] - q_starts[b] rows and L = seq_lens[b] tokens in the cache; its row i sees the keys 0 .. L - n + i.
 // o = sum_k softmax_k(q.k s) v; a row that sees nothing is zero. Softmax in one pass: running maximum and sum, fp32. The query heads of a kv head are
-// rows of one unit (row = token * G + head), so that a key is loaded once for the group. How the work is dealt out: paged_line.cuh. Up to 32 rows a
+// rows of one unit (row = token * G + head), so that a key is loaded once for the group. How the work is dealt out: paged_line.cuh. Up to 16 rows a
 // sequence: paged_few_attn.cu. This file: more rows, bound by the tensor cores and by the exponentials (16 a cycle and SM: 128 x 128 of them take as long as
 // the two products of a tile).
 //
@@ -559,7 +559,7 @@ void launch(LineParams p, int num_sms, void* scratch, cudaStream_t s) {
   using S = Shape<D, k8>;
   p.tile_tokens = 128 / p.G;
   p.tokens = 2 * p.tile_tokens;
-  place_scratch(p, scratch, num_sms, 0, S::kRows, D);
+  place_scratch(p, scratch, num_sms, S::kRows);
   const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.a.Hq), static_cast<uint64_t>(p.a.Tq)};
   const uint64_t pitch[2] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.a.ldq)};
   const uint32_t box[3] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.tile_tokens)};
@@ -579,20 +579,19 @@ void launch(LineParams p, int num_sms, void* scratch, cudaStream_t s) {
   launch_combine<D>(p, num_sms, s);
 }
 
-// Rows of a unit: 8 or 16 (the kernel of few rows) where the sequences have few on average, else 256. Up to 32 rows take two units of 16, of which the
-// second finds its keys in L2.
+// Rows of a unit: 8 or 16 (the kernel of few rows) where the sequences have so many on average, else 256. (32 sequences of 2 to 6 rows of a group of 7 over 500
+// - 4000 tokens, bf16: 46 us here, 62 us in units of 16.)
 int unit_rows(const ChunkAttnArgs& a, const PagedCache& c) {
   const int G = a.Hq / c.Hkv;
   const long long rows = static_cast<long long>(a.Tq) * G;
   if (G <= 8 && rows <= 8ll * a.B) return 8;
-  return G <= 16 && rows <= 32ll * a.B ? 16 : 256;
+  return G <= 16 && rows <= 16ll * a.B ? 16 : 256;
 }
 
 }  // namespace
 
 long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, int num_sms) {
-  const int rows = unit_rows(a, c);
-  return rows <= 16 ? paged_few_attn_scratch(rows, c, num_sms) : line_scratch(num_sms, 0, rows, c.D);
+  return line_scratch(num_sms, unit_rows(a, c), c.D);
 }
 
 void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int num_sms, void* scratch, cudaStream_t s) {

@@ -74,6 +74,9 @@ template <int D, bool k8, int kN>
 struct Few {
   static constexpr int kRows = 8 * kN;
   static constexpr int kWarps = kN == 1 ? (k8 ? 16 : 12) : (k8 ? 12 : 8);
+  static constexpr int kPartBytes = kWarps * 2 * kRows * D * 4;  // shared memory: the warps' parts, then (m, l); before that the line
+  static constexpr int kSmem = kPartBytes + kWarps * 2 * kRows * 8;
+  static_assert(kSmem >= 32768 && kSmem <= 232448 - 1024, "8192 sequences; shared memory");
 };
 
 struct Job {  // a unit whose parts this CTA's warps first .. last have
@@ -92,6 +95,8 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
   constexpr float kLift = k8 ? 7.f : 0.f;   // probabilities are held times 2^kLift
 
   extern __shared__ __align__(16) uint8_t shared[];
+  float* part_o = reinterpret_cast<float*>(shared);
+  float* part_ml = reinterpret_cast<float*>(shared + F::kPartBytes);
   __shared__ Job jobs[kW + 1];
   int* line = reinterpret_cast<int*>(shared);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -102,6 +107,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
   measure_line<kW * 32, kKeys>(p, line);
   const int worker = blockIdx.x * kW + warp;
   const Share share = find_share<kKeys, 2>(p, line, worker, gridDim.x * kW);
+  __syncthreads();  // the line is read, parts come there
   Walk<kKeys> w;
   w.start(p, share);
   if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -191,13 +197,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
       }
     };
     load_pages(w.j0);
-    {
-      const long long row = row_of(w.j0);
-      const int left = keys - w.j0 * kKeys;
-      load_k(std::true_type{}, left, row);
-      load_v(std::true_type{}, left, row);
-    }
-    // Q: rows g + 8 n, the dims of this lane's keys
+    // Q: rows g + 8 n, the dims of this lane's keys. Its loads go out while the pages are on their way.
     uint32_t q[kN][kSteps][2];
     float q_pow[kN][2];            // 8 bits: what rows 8 n + 2 t and 8 n + 2 t + 1 of S are to be multiplied with
 #pragma unroll
@@ -213,6 +213,15 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
         q[n][s][0] = x.x;
         q[n][s][1] = x.y;
       }
+    }
+    {
+      const long long row = row_of(w.j0);
+      const int left = keys - w.j0 * kKeys;
+      load_k(std::true_type{}, left, row);
+      load_v(std::true_type{}, left, row);
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
       if (k8) {
         uint32_t top = 0;
 #pragma unroll
@@ -432,7 +441,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
 
     // ---- the piece's end
     const bool whole = w.whole();
-    const long long part = static_cast<long long>(w.part(worker)) * F::kRows;
+    const int part = w.part(warp) * F::kRows;
     const float unit = k8 ? power(v_pow) : 1.f;
 #pragma unroll
     for (int n = 0; n < kN; ++n)
@@ -458,14 +467,14 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
             *reinterpret_cast<uint4*>(dst + (k8 ? D / 8 * g + 8 * i4 : 8 * g + 64 * i4)) = y;
           }
         } else {
-          float* dst = p.warp_o + (part + r) * D;
+          float* dst = part_o + (part + r) * D;
 #pragma unroll
           for (int i2 = 0; i2 < kSteps / 2; ++i2) {
             const int dim = k8 ? D / 8 * g + 4 * i2 : 8 * g + 64 * (i2 / 2) + 4 * (i2 % 2);
             *reinterpret_cast<float4*>(dst + dim) =
                 make_float4(o[n][2 * i2][i] * unit, o[n][2 * i2][i + 2] * unit, o[n][2 * i2 + 1][i] * unit, o[n][2 * i2 + 1][i + 2] * unit);
           }
-          if (g == 0) *reinterpret_cast<float2*>(p.warp_ml + (part + r) * 2) = make_float2(m[n][i], sum);
+          if (g == 0) *reinterpret_cast<float2*>(part_ml + (part + r) * 2) = make_float2(m[n][i], sum);
         }
       }
     // A unit that starts in this warp and goes on, or that goes on from the CTA before: its parts in this CTA are added below.
@@ -488,8 +497,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
     const int r = i % F::kRows;
     if (r >= job.tokens * G) continue;
     float o[D / 32], M, L;
-    const int base = blockIdx.x * kW;
-    add_parts<D>(p.warp_ml, p.warp_o, F::kRows, r, base + job.first, base + job.last, job.head, o, M, L);
+    add_parts<D, true>(part_ml, part_o, F::kRows, r, job.first, job.last, job.head, o, M, L);
     const bool here = job.end == static_cast<int>(blockIdx.x);
     if (here && job.head == 1) {
       store_row<D>(p, job.row0, job.kvh, r, o, L);
@@ -509,19 +517,14 @@ template <int D, bool k8, int kN>
 void launch(LineParams p, int num_sms, void* scratch, cudaStream_t s) {
   using F = Few<D, k8, kN>;
   p.tokens = p.tile_tokens = F::kRows / p.G;
-  place_scratch(p, scratch, num_sms, F::kWarps, F::kRows, D);
+  place_scratch(p, scratch, num_sms, F::kRows);
   auto kernel = paged_few_attn_kernel<D, k8, kN>;
-  launch_kernel(kernel, dim3(num_sms), dim3(F::kWarps * 32), p.a.B * 4, s, "paged_few_attn", p);  // B <= 8192: 32 KB
+  AGRPO_SET_MAX_DYN_SMEM(kernel, F::kSmem, "paged_few_attn smem attr");
+  launch_kernel(kernel, dim3(num_sms), dim3(F::kWarps * 32), F::kSmem, s, "paged_few_attn", p);
   launch_combine<D>(p, num_sms, s);
 }
 
 }  // namespace
-
-long long paged_few_attn_scratch(int rows, const PagedCache& c, int num_sms) {
-  const bool k8 = c.k_scale != nullptr;
-  const int warps = rows <= 8 ? (k8 ? Few<128, true, 1>::kWarps : Few<128, false, 1>::kWarps) : (k8 ? Few<128, true, 2>::kWarps : Few<128, false, 2>::kWarps);
-  return line_scratch(num_sms, warps, rows <= 8 ? 8 : 16, c.D);
-}
 
 void launch_paged_few_attn(const ChunkAttnArgs& a, const PagedCache& c, int rows, int num_sms, void* scratch, cudaStream_t s) {
   LineParams p = {};

@@ -27,8 +27,6 @@ struct LineParams {
   int4* desc;         // [CTAs]: the unit that starts in the CTA and ends in a later one {first row, tokens, kv head, last CTA}
   float* part_ml;     // [CTAs, 2, rows, 2]: parts, [0] of a unit that an earlier CTA starts, [1] of one that starts here
   float* part_o;      // [CTAs, 2, rows, D]
-  float* warp_ml;     // the same of warps, where those are the workers
-  float* warp_o;
 };
 
 struct Seq {
@@ -61,6 +59,7 @@ struct Share {
   int b, kvh, qb, j;   // sequence, kv head, unit, tile
   int tiles, before;   // of the share, ahead of it
   int total, workers;  // of the line; that have a share
+  Seq s;
 };
 
 // A worker's walk along its share: one piece (tiles [j0, j1) of a unit) after the other.
@@ -75,10 +74,8 @@ struct Walk {
     qb = at.qb;
     j0 = at.j;
     left = at.tiles;
-    if (left > 0) {
-      s = load_seq(p, b);
-      clip(p);
-    }
+    s = at.s;
+    if (left > 0) clip(p);
   }
   __device__ __forceinline__ bool more() const { return left > 0; }
   __device__ __forceinline__ void clip(const LineParams& p) {
@@ -160,27 +157,36 @@ __device__ __forceinline__ void measure_line(const LineParams& p, int* line) {
   __syncthreads();
 }
 
+// floor(total * i / n), without a 64-bit division.
+__device__ __forceinline__ int share_start(int total, int i, int n) {
+  const unsigned per = static_cast<unsigned>(total) / n, rest = static_cast<unsigned>(total) - per * n;
+  return static_cast<int>(per * i + rest * i / n);  // i and n are at most a few thousand
+}
+
 // A worker's share, of kLeast tiles at least if there are so many. One warp, all lanes with the same result.
 template <int kKeys, int kLeast>
 __device__ __forceinline__ Share find_share(const LineParams& p, const int* line, int worker, int workers) {
   const int lane = threadIdx.x & 31;
-  Share at = {0, 0, 0, 0, 0, 0, line[p.a.B - 1], 0};
+  Share at = {0, 0, 0, 0, 0, 0, line[p.a.B - 1], 0, {0, 0, 0, false}};
   at.workers = min(workers, (at.total + kLeast - 1) / kLeast);
   if (worker >= at.workers) return at;
-  at.before = static_cast<int>(static_cast<long long>(at.total) * worker / at.workers);
-  at.tiles = static_cast<int>(static_cast<long long>(at.total) * (worker + 1) / at.workers) - at.before;
-  int hi = p.a.B - 1;
-  while (at.b < hi) {
-    const int mid = (at.b + hi) / 2;
-    if (line[mid] > at.before) hi = mid;
-    else at.b = mid + 1;
+  at.before = share_start(at.total, worker, at.workers);
+  at.tiles = share_start(at.total, worker + 1, at.workers) - at.before;
+  // The sequence: first the one of up to 32 groups, then within it.
+  for (int first = 0, many = p.a.B; many > 1;) {
+    const int step = (many + 31) / 32, end = min(first + (lane + 1) * step, first + many);  // lane i: up to the end of group i
+    const unsigned past = __ballot_sync(0xffffffffu, line[end - 1] > at.before);
+    const int group = __ffs(past) - 1;
+    many = min(step, many - group * step);
+    first += group * step;
+    at.b = first;
   }
   const int ahead = at.b > 0 ? line[at.b - 1] : 0;
   const int per = (line[at.b] - ahead) / p.c.Hkv;
   int r = at.before - ahead;
   at.kvh = r / per;
   r -= at.kvh * per;
-  const Seq s = load_seq(p, at.b);
+  const Seq s = at.s = load_seq(p, at.b);
   for (int q0 = 0; q0 < num_units(p, s); q0 += 32) {
     const int q = q0 + lane;
     const int nk = q < num_units(p, s) ? unit_tiles<kKeys>(p, s, q) : 0;
@@ -204,7 +210,7 @@ __device__ __forceinline__ Share find_share(const LineParams& p, const int* line
 
 // One row's share of a unit: adds the parts first .. last (the first in place `head` of its pair, the others in 0). A warp; lane i gets dims i D / 32 and on, and
 // every lane the row's maximum and sum.
-template <int D>
+template <int D, bool kShared>
 __device__ __forceinline__ void add_parts(const float* part_ml, const float* part_o, int rows, int row, int first, int last, int head, float (&o)[D / 32], float& M,
                                           float& L) {
   constexpr int kPer = D / 32;
@@ -215,7 +221,8 @@ __device__ __forceinline__ void add_parts(const float* part_ml, const float* par
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
   for (int k0 = first; k0 <= last; k0 += 32) {
     const int k = min(k0 + lane, last);
-    float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + ((static_cast<long long>(k) * 2 + (k == first ? head : 0)) * rows + row) * 2));
+    const auto* at = reinterpret_cast<const float2*>(part_ml + ((static_cast<long long>(k) * 2 + (k == first ? head : 0)) * rows + row) * 2);
+    float2 ml = kShared ? *at : __ldcg(at);
     if (k0 + lane > last) ml.y = 0.f;
     float mx = ml.y != 0.f ? ml.x : -INFINITY;
 #pragma unroll
@@ -237,8 +244,8 @@ __device__ __forceinline__ void add_parts(const float* part_ml, const float* par
       for (int i = 0; i < 8; ++i) {
         const int part = min(k0 + i0 + i, last);
         const float* src = part_o + ((static_cast<long long>(part) * 2 + (part == first ? head : 0)) * rows + row) * D + lane * kPer;
-        if (kPer == 4) *reinterpret_cast<float4*>(x[i]) = __ldcg(reinterpret_cast<const float4*>(src));
-        else *reinterpret_cast<float2*>(x[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+        if (kPer == 4) *reinterpret_cast<float4*>(x[i]) = kShared ? *reinterpret_cast<const float4*>(src) : __ldcg(reinterpret_cast<const float4*>(src));
+        else *reinterpret_cast<float2*>(x[i]) = kShared ? *reinterpret_cast<const float2*>(src) : __ldcg(reinterpret_cast<const float2*>(src));
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -276,25 +283,33 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const LineParams p) 
   if (r >= u.y * p.G) return;
   const int tile = r / p.G / p.tile_tokens;  // a tile's rows start on 128
   float o[D / 32], M, L;
-  add_parts<D>(p.part_ml, p.part_o, p.rows, r + tile * (128 - p.tile_tokens * p.G), c, u.w, 1, o, M, L);
+  add_parts<D, false>(p.part_ml, p.part_o, p.rows, r + tile * (128 - p.tile_tokens * p.G), c, u.w, 1, o, M, L);
   store_row<D>(p, u.x, u.z, r, o, L);
 }
 
 // Workspace of a launch: what LineParams points to.
-inline long long line_scratch(int ctas, int warps, int rows, int D) { return ctas * 16ll + static_cast<long long>(ctas) * (1 + warps) * 2 * rows * (2 + D) * 4; }
-inline void place_scratch(LineParams& p, void* scratch, int ctas, int warps, int rows, int D) {
+inline long long line_scratch(int ctas, int rows, int D) { return static_cast<long long>(ctas) * (16 + 2 * rows * (2 + D) * 4); }
+inline void place_scratch(LineParams& p, void* scratch, int ctas, int rows) {
   p.rows = rows;
   p.desc = static_cast<int4*>(scratch);
   p.part_ml = reinterpret_cast<float*>(p.desc + ctas);
   p.part_o = p.part_ml + static_cast<long long>(ctas) * 2 * rows * 2;
-  p.warp_ml = p.part_o + static_cast<long long>(ctas) * 2 * rows * D;
-  p.warp_o = p.warp_ml + static_cast<long long>(ctas) * warps * 2 * rows * 2;
 }
+// Always a dependent launch: its own start overlaps the end of the kernel before it, on whose completion it waits.
 template <int D>
 inline void launch_combine(const LineParams& p, int ctas, cudaStream_t s) {
   auto combine = paged_combine_kernel<D>;
   AGRPO_PREFER_SMEM(combine);
-  launch_kernel(combine, dim3(ctas, (p.rows + 7) / 8), dim3(256), 0, s, "paged_combine", p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, (p.rows + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, combine, p), "paged_combine");
 }
 
 }  // namespace

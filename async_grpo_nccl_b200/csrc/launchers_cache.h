@@ -44,7 +44,6 @@ long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, 
 void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int num_sms, void* scratch, cudaStream_t s);
 
 // Its form for units of up to 8 or 16 rows (paged_few_attn.cu).
-long long paged_few_attn_scratch(int rows, const PagedCache& c, int num_sms);
 void launch_paged_few_attn(const ChunkAttnArgs& a, const PagedCache& c, int rows, int num_sms, void* scratch, cudaStream_t s);
 
 }  // namespace agrpo
