@@ -31,6 +31,8 @@ constexpr int kBN = 128;  // keys a tile
 template <int D>
 constexpr int kGroupBytes = D / 64 * 1024;
 
+constexpr int kSeqRoom = 128;  // sequences that a CTA has at hand
+
 template <int D, bool k8>
 struct Shape {
   static constexpr int kRows = 256;                           // rows of a unit
@@ -45,7 +47,8 @@ struct Shape {
   static constexpr int kRawOff = kRingOff + kSlots * kSlotBytes;
   static constexpr int kScaleOff = kRawOff + kRaw * kBN * D;
   static constexpr int kBarOff = kScaleOff + kRaw * kBN;
-  static constexpr int kSmem = kBarOff + 256 + 1024;          // with room to align
+  static constexpr int kSeqOff = kBarOff + 256;
+  static constexpr int kSmem = kSeqOff + kSeqRoom * 12 + 1024;  // with room to align
   static_assert(kSmem <= 232448, "shared memory");
   static_assert(kSlots * kSlotBytes >= 32768, "the line of 8192 sequences is measured in the ring's memory");
 };
@@ -121,13 +124,15 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   pdl_launch();
   measure_line<S::kThreads, kBN>(p, reinterpret_cast<int*>(ring));
   const Share share = find_share<kBN, 1>(p, reinterpret_cast<const int*>(ring), blockIdx.x, gridDim.x);
+  const SeqCache near = {reinterpret_cast<int*>(smem + S::kSeqOff), share.b, kSeqRoom};
+  near.fill(p);
   fence_proxy_async_smem();  // the line lies where the ring's copies go next
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Walk<kBN> w;  // every warp walks by itself
-  w.start(p, share);
+  w.start(p, share, near);
 
   if (warp == S::kLoadWarp) {
     give_registers<k8, 72>();
@@ -505,6 +510,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       tc_fence_after();
       if (busy) {
         const bool whole = w.whole(), valid = r < rows;
+        // a lane's stores are a row of their own: whole 32-byte sectors where the output's rows allow it
+        const bool wide = ((reinterpret_cast<uintptr_t>(p.a.out) | static_cast<uintptr_t>(p.a.ldo * 2)) & 31) == 0;
         const float inv = l != 0.f ? 1.f / l : 0.f;
         const long long part = static_cast<long long>(w.part(blockIdx.x)) * S::kRows + t * 128 + r;
         auto* dst = static_cast<__nv_bfloat16*>(p.a.out) + (w.s.row0 + w.qb * p.tokens + t * p.tile_tokens + r_tok) * p.a.ldo +
@@ -520,18 +527,25 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           }
           if (valid && whole) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 y;
-              y.x = pack_bf16x2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-              y.y = pack_bf16x2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-              y.z = pack_bf16x2(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-              y.w = pack_bf16x2(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + c * 32 + i) = y;
+            for (int i = 0; i < 32; i += 16) {
+              uint32_t y[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) y[k] = pack_bf16x2(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+              if (wide) {
+                st_global_32b(dst + c * 32 + i, y);
+              } else {
+                *reinterpret_cast<uint4*>(dst + c * 32 + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(dst + c * 32 + i + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+              }
             }
           } else if (valid) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(p.part_o + part * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t y[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) y[k] = o[i + k];
+              st_global_32b(p.part_o + part * D + c * 32 + i, y);
+            }
           }
         }
         if (valid && !whole) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);

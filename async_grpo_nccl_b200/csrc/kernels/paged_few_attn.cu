@@ -32,6 +32,7 @@ namespace agrpo {
 namespace {
 
 constexpr int kKeys = 16;
+constexpr int kSeqRoom = 128;      // sequences that a CTA has at hand
 constexpr float kNone = -3.0e38f;  // maximum of nothing: finite, so that a difference with it is a number
 
 template <bool half>
@@ -76,7 +77,7 @@ struct Few {
   static constexpr int kWarps = kN == 1 ? (k8 ? 16 : 12) : (k8 ? 12 : 8);
   static constexpr int kPartBytes = kWarps * 2 * kRows * D * 4;  // shared memory: the warps' parts, then (m, l); before that the line
   static constexpr int kSmem = kPartBytes + kWarps * 2 * kRows * 8;
-  static_assert(kSmem >= 32768 && kSmem <= 232448 - 1024, "8192 sequences; shared memory");
+  static_assert(kSmem >= 32768 && kSmem <= 232448 - 1024 - kSeqRoom * 12, "8192 sequences; shared memory");
 };
 
 struct Job {  // a unit whose parts this CTA's warps first .. last have
@@ -107,9 +108,14 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
   measure_line<kW * 32, kKeys>(p, line);
   const int worker = blockIdx.x * kW + warp;
   const Share share = find_share<kKeys, 2>(p, line, worker, gridDim.x * kW);
+  __shared__ int seqs[3 * kSeqRoom], first_seq;
+  if (threadIdx.x == 0) first_seq = share.b;
   __syncthreads();  // the line is read, parts come there
+  const SeqCache near = {seqs, first_seq, kSeqRoom};
+  near.fill(p);
+  __syncthreads();
   Walk<kKeys> w;
-  w.start(p, share);
+  w.start(p, share, near);
   if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
 
   const int bs = p.c.block_size, Hkv = p.c.Hkv, G = p.G;

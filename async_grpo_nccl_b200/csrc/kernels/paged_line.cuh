@@ -46,6 +46,24 @@ __device__ __forceinline__ Seq load_seq(const LineParams& p, int b) {
   }
   return s;
 }
+// The sequences from a CTA's first one on, in shared memory: a walk that had to load the next one would stop for it.
+struct SeqCache {
+  int* at;           // {row0, n, len} of each
+  int first, room;
+  __device__ __forceinline__ void fill(const LineParams& p) const {  // all threads; synchronise after it
+    for (int i = threadIdx.x; i < room && first + i < p.a.B; i += blockDim.x) {
+      const Seq s = load_seq(p, first + i);
+      at[3 * i] = s.row0;
+      at[3 * i + 1] = s.n;
+      at[3 * i + 2] = s.len;
+    }
+  }
+  __device__ __forceinline__ Seq get(const LineParams& p, int b) const {
+    const int i = b - first;
+    if (i >= room) return load_seq(p, b);
+    return Seq{at[3 * i], at[3 * i + 1], at[3 * i + 2], false};
+  }
+};
 // Keys that the last row of unit qb sees, and tiles of them. A unit without keys still has a tile: its rows are zeros to be written.
 __device__ __forceinline__ int unit_keys(const LineParams& p, const Seq& s, int qb) { return max(s.len - s.n + min(s.n, (qb + 1) * p.tokens), 0); }
 template <int kKeys>
@@ -66,9 +84,11 @@ struct Share {
 template <int kKeys>
 struct Walk {
   Seq s;
+  SeqCache near;
   int b, kvh, qb, j0, j1, nk, left;
 
-  __device__ __forceinline__ void start(const LineParams& p, const Share& at) {
+  __device__ __forceinline__ void start(const LineParams& p, const Share& at, const SeqCache& cache) {
+    near = cache;
     b = at.b;
     kvh = at.kvh;
     qb = at.qb;
@@ -90,7 +110,7 @@ struct Walk {
       qb = 0;
       if (++kvh == p.c.Hkv) {
         kvh = 0;
-        do s = load_seq(p, ++b);
+        do s = near.get(p, ++b);
         while (s.n == 0);
       }
     }
@@ -288,11 +308,11 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const LineParams p) 
 }
 
 // Workspace of a launch: what LineParams points to.
-inline long long line_scratch(int ctas, int rows, int D) { return static_cast<long long>(ctas) * (16 + 2 * rows * (2 + D) * 4); }
+inline long long line_scratch(int ctas, int rows, int D) { return static_cast<long long>(ctas) * (32 + 2 * rows * (2 + D) * 4); }
 inline void place_scratch(LineParams& p, void* scratch, int ctas, int rows) {
   p.rows = rows;
   p.desc = static_cast<int4*>(scratch);
-  p.part_ml = reinterpret_cast<float*>(p.desc + ctas);
+  p.part_ml = reinterpret_cast<float*>(p.desc + 2 * ctas);  // everything on 32 bytes
   p.part_o = p.part_ml + static_cast<long long>(ctas) * 2 * rows * 2;
 }
 // Always a dependent launch: its own start overlaps the end of the kernel before it, on whose completion it waits.
