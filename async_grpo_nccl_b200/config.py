@@ -57,6 +57,8 @@ class GRPOConfig:
     enable_prefix_caching: bool = True  # full prompt blocks stay findable by the hash of their token chain until the next weight push
     vllm_engine_preset: str = "eager"  # "eager" | "throughput" (CUDA-graphed decode step)
     kv_block_size: int = 16
+    kv_cache_dtype: str = "auto"  # "auto": bf16 | "fp8": e4m3 codes with a power of two for each token and kv head, half the bytes
+    prefill_chunk_tokens: int = 0  # > 0: prompts go through the rollout engine in portions of at most so many tokens
     gpu_memory_utilization: float = 0.90
     # ---- verifier / rewards ----
     global_num_verifiers: int = 4
@@ -184,6 +186,10 @@ class GRPOConfig:
         need(self.temperature >= 0.0, "temperature must be non-negative")
         need(self.lr_scheduler in ("constant", "cosine", "constant_with_warmup"), "unknown lr_scheduler")
         need(self.vllm_engine_preset in ("eager", "throughput"), "vllm_engine_preset must be eager or throughput")
+        need(self.kv_cache_dtype in ("auto", "fp8"), "kv_cache_dtype must be auto or fp8")
+        need(self.prefill_chunk_tokens >= 0, "prefill_chunk_tokens must be >= 0")
+        need(self.generation_tp_size == 1 or (self.kv_cache_dtype == "auto" and self.prefill_chunk_tokens == 0),
+             "a tensor-parallel rollout replica has neither an 8-bit cache nor prompts in portions")
         need(self.colocated_sm_limit >= 0, "colocated_sm_limit must be >= 0")
         need(self.colocated_rollout_sms >= 0, "colocated_rollout_sms must be >= 0")
         need(self.param_sharding in ("zero2", "zero3", "auto"), "param_sharding must be zero2/zero3/auto")

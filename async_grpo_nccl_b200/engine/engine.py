@@ -7,6 +7,7 @@ prefetched once; only its partial last block is copied per sample).
 
 * scheduling / block accounting: C++ (``csrc/host/kv_allocator.cpp``)
 * prefill: packed varlen forward through the same decoder kernels as training, K/V written to the pages
+  (optionally in portions that attend over the pages, ``prefill_chunk_tokens``)
 * decode: one fused step per token for all running sequences (skinny tcgen05 GEMMs, paged-KV GQA
   attention, lm_head + Gumbel-max sampling without materialising logits), optionally replayed from a
   CUDA graph (preset ``throughput``)
@@ -67,11 +68,13 @@ class RolloutEngine:
     def __init__(self, cfg: ModelConfig, layout: ParamLayout, params: torch.Tensor, *, max_seqs: int = 256,
                  max_model_len: Optional[int] = None, num_blocks: Optional[int] = None, block_size: int = 16,
                  kv_memory_bytes: Optional[int] = None, max_prefill_tokens: int = 16384, use_cuda_graph: bool = False,
-                 eos_token_id: Optional[int] = None, tp: Any = None, prefix_caching: bool = False):
+                 eos_token_id: Optional[int] = None, tp: Any = None, prefix_caching: bool = False, kv_cache_dtype: str = "auto",
+                 prefill_chunk_tokens: int = 0):
         from ..ops import native
 
         assert params.is_cuda
         self._check_model(cfg, params, block_size)
+        self._init_cache_kind(kv_cache_dtype, int(prefill_chunk_tokens))
         self.C = native()
         self.cfg, self.layout, self.params = cfg, layout, params
         self.dev = params.device
@@ -125,6 +128,19 @@ class RolloutEngine:
         if block_size != 16 or cfg.head_dim != 128:
             raise ValueError("the native engine supports block_size 16 and head_dim 128")
 
+    def _init_cache_kind(self, kv_cache_dtype: str, prefill_chunk_tokens: int) -> None:
+        """``kv_cache_dtype`` "fp8": keys and values are kept as e4m3 codes with a power of two for each token and kv head, half the bytes
+        of bf16 ("auto"): twice the tokens in the same memory, half the traffic of a decode step, and values of three mantissa bits. Prompts
+        then attend over the pages as well, so that a token's keys are the same bits for everyone who reads them.
+        ``prefill_chunk_tokens`` > 0: prompts go through the layers in portions of at most so many tokens, each attending over the
+        pages; activation memory is bounded whatever the prompt's length."""
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype must be 'auto' or 'fp8', not {kv_cache_dtype!r}")
+        if prefill_chunk_tokens < 0:
+            raise ValueError("prefill_chunk_tokens must be >= 0")
+        self.kv8 = kv_cache_dtype == "fp8"
+        self.prefill_chunk_tokens = prefill_chunk_tokens
+
     def _init_sharing(self, tp: Any, prefix_caching: bool) -> None:
         cfg = self.cfg
         # Tensor parallelism (vllm_worker.py:219-232, tensor_parallel_size): ``tp`` is a parallel.symm.TensorParallelComm.
@@ -145,18 +161,26 @@ class RolloutEngine:
         # reuses them and only its remaining tokens go through the GEMMs. Forgotten at every weight update. A
         # tensor-parallel member caches only its own kv heads while the prefill needs all of them, so it stays off there.
         self.prefix_caching = bool(prefix_caching) and self.tp is None
+        if self.tp is not None and (self.kv8 or self.prefill_chunk_tokens > 0):
+            # likewise: a member's pages do not hold the heads that its part of the prefill attends over
+            raise ValueError("a tensor-parallel replica has neither an 8-bit cache nor prompts in portions")
 
     def _init_decoder(self) -> None:
         self.dec = NativeDecoder(self.cfg, self.layout, self.params)
         self.dec.ensure_rope(min(self.max_model_len, self.cfg.max_position_embeddings))
 
     def _bytes_per_block(self) -> int:
-        return self.cfg.num_hidden_layers * 2 * self.Hkv_l * self.block_size * self.cfg.head_dim * 2
+        return self.cfg.num_hidden_layers * 2 * self.Hkv_l * self.block_size * (self.cfg.head_dim + 1 if self.kv8 else self.cfg.head_dim * 2)
 
     def _alloc_cache(self) -> None:
         cfg = self.cfg
-        self.cache = torch.zeros(cfg.num_hidden_layers, 2, self.num_blocks, self.Hkv_l, self.block_size,
-                                 cfg.head_dim, dtype=torch.bfloat16, device=self.dev)
+        shape = (cfg.num_hidden_layers, 2, self.num_blocks, self.Hkv_l, self.block_size)
+        self.cache_scale: Optional[torch.Tensor] = None
+        if self.kv8:
+            self.cache = torch.zeros(*shape, cfg.head_dim, dtype=torch.uint8, device=self.dev).view(torch.float8_e4m3fn)
+            self.cache_scale = torch.full(shape, 127, dtype=torch.uint8, device=self.dev)
+        else:
+            self.cache = torch.zeros(*shape, cfg.head_dim, dtype=torch.bfloat16, device=self.dev)
 
     def _window_tokens(self) -> int:
         """How far back any layer looks (0 = to the start): blocks beyond it go back to the pool."""
@@ -222,6 +246,7 @@ class RolloutEngine:
         self.b_attn = torch.zeros(SA, self.qd_l, **bf)
         self.b_gu = torch.empty(S, 2 * self.F_l, **bf)
         self.b_act = torch.zeros(SA, self.F_l, **bf)
+        self.b_starts = torch.arange(S + 1, **i32)  # 8 bits: one row a sequence
         self.max_splits = 8
         self.b_part_o = torch.empty(S * cfg.num_key_value_heads * self.max_splits * 8 * cfg.head_dim, dtype=torch.float32,
                                     device=self.dev)
@@ -251,7 +276,7 @@ class RolloutEngine:
         self.mega_rows = 0
         self.mega_trace: Optional[torch.Tensor] = None  # int64[32]: phase stamps of CTA 0 in layer mega_trace_layer
         self.mega_trace_layer = 0
-        if (self.fused_decode and self.tp is None and os.environ.get("AGRPO_DECODE_MEGA", "1") != "0"
+        if (self.fused_decode and self.tp is None and not self.kv8 and os.environ.get("AGRPO_DECODE_MEGA", "1") != "0"
                 and self.C.decode_layers_supported(min(256, S), H, Q, cfg.q_dim, F, cfg.num_attention_heads,
                                                    cfg.num_key_value_heads, cfg.head_dim)):
             # It wins where the step is latency-bound: up to 32 rows 1.36 against 1.71 ms at 600 tokens of context, 1.46 to 1.56
@@ -332,6 +357,10 @@ class RolloutEngine:
     def _vc(self, i: int) -> torch.Tensor:
         return self.cache[i, 1]
 
+    def _scales(self, i: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """Scale bytes of layer i's keys and values (8 bits)."""
+        return (self.cache_scale[i, 0], self.cache_scale[i, 1]) if self.cache_scale is not None else (None, None)
+
     def _apply_table_updates(self, plan: Dict[str, Any]) -> None:
         n = len(plan["upd_slot"])
         if n == 0:
@@ -350,6 +379,11 @@ class RolloutEngine:
     def _prompt_hidden(self, plan: Dict[str, Any], reqs: List[_Request]) -> torch.Tensor:
         """Runs the prompts of a prefill plan; returns the normalised hidden state of every prompt's last token."""
         cfg, C, dec = self.cfg, self.C, self.dec
+        if self.kv8 or self.prefill_chunk_tokens > 0:
+            xl = self._prefill_portions(plan, reqs)
+            hn = torch.empty_like(xl)
+            C.rmsnorm_fwd(xl, dec.w("final_norm"), hn, None, cfg.rms_norm_eps)
+            return hn
         samples = [{"sample_ids": r.prompt, "input_len": len(r.prompt), "output_len": 0, "advantage": 0.0} for r in reqs]
         host_batch = pack_samples(samples, pin=True)
         batch = host_batch.to_device(self.dev)
@@ -375,8 +409,58 @@ class RolloutEngine:
         C.rmsnorm_fwd(xl, dec.w("final_norm"), hn, None, cfg.rms_norm_eps)
         return hn
 
+    def _prefill_portions(self, plan: Dict[str, Any], reqs: List[_Request]) -> torch.Tensor:
+        """The tokens of a plan's prompts that are not in the cache yet, in portions of at most ``prefill_chunk_tokens`` (or
+        ``max_prefill_tokens``): a portion's keys and values go into the pages layer by layer, and its rows attend over the pages. Returns the
+        hidden state of every prompt's last token."""
+        cfg, C, dec = self.cfg, self.C, self.dec
+        self._apply_table_updates(plan)
+        cos_t, sin_t = dec.rope_tables(1)
+        cached = list(plan.get("cached_lens") or [0] * len(reqs))
+        lens = [len(r.prompt) for r in reqs]
+        if self.prefix_caching:
+            self.prefix_lookup_tokens += sum(lens)
+            self.prefix_hit_tokens += int(sum(cached))
+        ids = np.concatenate([r.prompt[c:] for r, c in zip(reqs, cached)])
+        pos = np.concatenate([np.arange(c, n, dtype=np.int32) for n, c in zip(lens, cached)])
+        first = np.cumsum([0] + [n - c for n, c in zip(lens, cached)])           # row of every prompt's first new token
+        size = self.prefill_chunk_tokens or self.max_prefill_tokens
+        portions, words = [], [ids.astype(np.int32), pos, np.asarray(plan["slot_mapping"], dtype=np.int32),
+                               np.cumsum([0] + [r.n for r in reqs[:-1]]).astype(np.int32)]
+        n_rows, at = len(ids), 3 * len(ids) + len(reqs)
+        for a in range(0, n_rows, size):
+            z = min(n_rows, a + size)
+            g0, g1 = int(np.searchsorted(first, a, "right")) - 1, int(np.searchsorted(first, z, "left"))
+            ends = np.minimum(first[g0 + 1:g1 + 1], z)                            # of the prompts' rows in this portion
+            starts = np.concatenate([[a], ends]) - a
+            upto = ends - first[g0:g1] + np.asarray(cached[g0:g1])               # tokens that the prompts have in the cache after it
+            done = [int(e) - a - 1 for e, f in zip(ends, first[g0 + 1:g1 + 1]) if e == f]
+            words += [starts.astype(np.int32), upto.astype(np.int32), np.asarray(done, dtype=np.int32)]
+            portions.append((a, z, g0, g1, at, len(done)))
+            at += len(starts) + len(upto) + len(done)
+        host = torch.from_numpy(np.concatenate(words)).pin_memory()
+        d = host.to(self.dev, non_blocking=True)
+        self.h2d_bytes += host.numel() * 4 + 16 * len(plan["seq_slots"])
+        # a request's first sample holds the prompt's pages
+        slots = torch.tensor(plan["seq_slots"], dtype=torch.int32).pin_memory().to(self.dev, non_blocking=True)
+        tables = self.block_tables.index_select(0, slots.index_select(0, d[3 * n_rows:3 * n_rows + len(reqs)]))
+        last: List[torch.Tensor] = []
+        for a, z, g0, g1, at, n_done in portions:
+            k = g1 - g0
+            starts, upto, done = d[at:at + k + 1], d[at + k + 1:at + 2 * k + 1], d[at + 2 * k + 1:at + 2 * k + 1 + n_done]
+            x = torch.empty(z - a, cfg.hidden_size, dtype=torch.bfloat16, device=self.dev)
+            C.embedding_fwd(d[a:z], dec.w("embed"), x)
+            for i in range(cfg.num_hidden_layers):
+                x = dec.layer_fwd_paged(i, x, d[n_rows + a:n_rows + z], cos_t, sin_t, self._kc(i), self._vc(i), *self._scales(i),
+                                        d[2 * n_rows + a:2 * n_rows + z], tables[g0:g1], upto, starts)
+            if n_done:
+                last.append(x.index_select(0, done))
+        dec.launches += len(portions)
+        return torch.cat(last, dim=0)
+
     def _copy_blocks(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        self.cache[:, :, dst] = self.cache[:, :, src]
+        for c in (self.cache.view(torch.uint8), self.cache_scale) if self.kv8 else (self.cache,):
+            c[:, :, dst] = c[:, :, src]
 
     def _share_prompt_state(self, plan: Dict[str, Any], reqs: List[_Request]) -> None:
         """The n samples of a prompt start from the same state: copies what they cannot share (the partial last block)."""
@@ -456,14 +540,14 @@ class RolloutEngine:
         n_p = int(sum(int(c) for c in cached))
         sfx, pfx = idx[:n_s], idx[n_s:n_s + n_p]
         last = idx[n_s + n_p:n_s + n_p + len(cached)]
-        pslots = idx[n_s + n_p + len(cached):]
+        pslots = torch.full((batch.T,), -1, dtype=torch.int32, device=self.dev)  # cached tokens' slots, at their rows
+        pslots[pfx] = idx[n_s + n_p + len(cached):].to(torch.int32)
         ids_s = batch.ids.index_select(0, sfx)
         pos_s = batch.pos.index_select(0, sfx)
         x = torch.empty(n_s, cfg.hidden_size, dtype=torch.bfloat16, device=self.dev)
         C.embedding_fwd(ids_s, dec.w("embed"), x)
-        blk, off = pslots // self.block_size, pslots % self.block_size
         for i in range(cfg.num_hidden_layers):
-            x = dec.layer_fwd_suffix(i, x, batch, sfx, pfx, pos_s, cos_t, sin_t, self._kc(i), self._vc(i), slots, blk, off)
+            x = dec.layer_fwd_suffix(i, x, batch, sfx, pslots, pos_s, cos_t, sin_t, self._kc(i), self._vc(i), slots)
         return x.index_select(0, last)
 
     def _decode_forward(self, B: int, temperature: float, splits: int) -> None:
@@ -482,7 +566,6 @@ class RolloutEngine:
         x, x1, h, qkv, attn, gu, act = (self.b_x[:B], self.b_x1[:B], self.b_h[:B], self.b_qkv[:B], self.b_attn[:B],
                                         self.b_gu[:B], self.b_act[:B])
         bt, sl = self.block_tables, self.seq_lens
-        scale = 1.0 / math.sqrt(cfg.head_dim)
         C.embedding_fwd(self.last_tokens[:B], dec.w("embed"), x)
         for i in range(cfg.num_hidden_layers):
             p = f"layers.{i}."
@@ -490,9 +573,8 @@ class RolloutEngine:
             C.gemm_bf16(h, dec.w(p + "wqkv"), qkv, False, False, dec.w(p + "bqkv") if cfg.attention_bias else None, 1.0, False,
                         self.status, None)
             C.rope_kv_write_decode(qkv, cos_t, sin_t, bt, sl, self._kc(i), self._vc(i), cfg.num_attention_heads,
-                                   cfg.num_key_value_heads, cfg.head_dim, self.status)
-            C.paged_decode_attn(qkv, self._kc(i), self._vc(i), bt, sl, attn, cfg.num_attention_heads, cfg.num_key_value_heads,
-                                cfg.head_dim, scale, splits, self.b_part_o, self.b_part_ml, self.status, self.b_tickets)
+                                   cfg.num_key_value_heads, cfg.head_dim, self.status, *self._scales(i))
+            self._decode_attn(i, qkv, bt, sl, attn, splits)
             C.gemm_bf16(attn, dec.w(p + "wo"), x1, False, False, None, 1.0, False, self.status, x)
             C.rmsnorm_fwd(x1, dec.w(p + "ln2"), h, None, cfg.rms_norm_eps)
             C.gemm_bf16(h, dec.w(p + "wgu"), gu, False, False, None, 1.0, False, self.status, None)
@@ -502,6 +584,17 @@ class RolloutEngine:
         wl = self.layout.view(self.params, self.layout.lm_head_name())
         C.lm_sample(h, wl, temperature, self.step_seeds, self.b_sample_f, self.b_sample_i, self.b_tokens, self.b_lp, self.status)
         self._feed_back(B)
+
+    def _decode_attn(self, i: int, qkv: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, out: torch.Tensor, splits: int) -> None:
+        """Attention of one row a sequence over layer i's pages."""
+        cfg = self.cfg
+        scale = 1.0 / math.sqrt(cfg.head_dim)
+        if self.kv8:
+            self.C.paged_chunk_attn(qkv, self._kc(i), self._vc(i), tables, lens, self.b_starts[:qkv.shape[0] + 1], out, self.Hq_l, self.Hkv_l,
+                                    cfg.head_dim, scale, self.status, *self._scales(i))
+        else:
+            self.C.paged_decode_attn(qkv, self._kc(i), self._vc(i), tables, lens, out, self.Hq_l, self.Hkv_l, cfg.head_dim, scale, splits,
+                                     self.b_part_o, self.b_part_ml, self.status, self.b_tickets)
 
     def _feed_back(self, B: int) -> None:
         """The sampled token becomes the next step's input and goes into the history (with its log-probability when kept)."""
@@ -559,7 +652,6 @@ class RolloutEngine:
         cfg, C, dec = self.cfg, self.C, self.dec
         cos_t, sin_t = dec.rope_tables(1)
         ss = self.b_ss
-        scale = 1.0 / math.sqrt(cfg.head_dim)
         eps = cfg.rms_norm_eps
         st = self.status
         R = self.fused_chunk
@@ -580,14 +672,13 @@ class RolloutEngine:
                 x, x1, qkv, attn, act = (self.b_x[r0:r1], self.b_x1[r0:r1], self.b_qkv[r0:r1], self.b_attn[r0:r1], self.b_act[r0:r1])
                 bt, sl = self.block_tables[r0:r1], self.seq_lens[r0:r1]
                 s0, s1, s2 = ss[2 * i, r0:r1], ss[2 * i + 1, r0:r1], ss[2 * i + 2, r0:r1]
-                # up to 128 rows: rotary embedding and the KV-cache write happen in the qkv GEMM's epilogue
-                ok = (r1 - r0) <= 128 and C.gemm_decode_rope(x, fq, qkv, bq, s0, eps, cos_t, sin_t, bt, sl, self._kc(i), self._vc(i),
+                # up to 128 rows: rotary embedding and the KV-cache write happen in the qkv GEMM's epilogue (bf16 cache)
+                ok = not self.kv8 and (r1 - r0) <= 128 and C.gemm_decode_rope(x, fq, qkv, bq, s0, eps, cos_t, sin_t, bt, sl, self._kc(i), self._vc(i),
                                                              Hq, Hkv, st)
                 if not ok:
                     ok = C.gemm_decode(x, fq, qkv, bq, None, s0, None, eps, st)
-                    C.rope_kv_write_decode(qkv, cos_t, sin_t, bt, sl, self._kc(i), self._vc(i), Hq, Hkv, cfg.head_dim, st)
-                C.paged_decode_attn(qkv, self._kc(i), self._vc(i), bt, sl, attn, Hq, Hkv,
-                                    cfg.head_dim, scale, splits, self.b_part_o, self.b_part_ml, st, self.b_tickets)
+                    C.rope_kv_write_decode(qkv, cos_t, sin_t, bt, sl, self._kc(i), self._vc(i), Hq, Hkv, cfg.head_dim, st, *self._scales(i))
+                self._decode_attn(i, qkv, bt, sl, attn, splits)
                 if tp is None:
                     ok = C.gemm_decode(attn, wo, x1, None, x, None, s1, eps, st) and ok
                     C.gemm_swiglu(x1, fg, act, s1, eps, st)
@@ -641,12 +732,14 @@ class RolloutEngine:
         if self.mega_rows and 0 < B <= self.mega_rows:
             return 1 + 1 + 4
         fused = self.fused_decode and 0 < B <= self.fused_rows
-        if fused:
+        if fused and self.kv8:
+            per_layer = 7 * ((B + self.fused_chunk - 1) // self.fused_chunk)
+        elif fused:
             n_chunks = (B + self.fused_chunk - 1) // self.fused_chunk
             last = B - (n_chunks - 1) * self.fused_chunk
             per_layer = (n_chunks - 1) * (5 if self.fused_chunk <= 128 else 6) + (5 if last <= 128 else 6)
         else:
-            per_layer = 9
+            per_layer = 9 + self.kv8
         return 1 + per_layer * self.cfg.num_hidden_layers + 4
 
     def _stage_decode(self, active: np.ndarray, upd_slot: np.ndarray, upd_index: np.ndarray, upd_block: np.ndarray) -> None:

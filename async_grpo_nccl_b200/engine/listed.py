@@ -31,6 +31,12 @@ class ListedEngine(RolloutEngine):
         if block_size != 16:
             raise ValueError("the engine supports block_size 16")
 
+    def _init_cache_kind(self, kv_cache_dtype: str, prefill_chunk_tokens: int) -> None:
+        if kv_cache_dtype != "auto" or prefill_chunk_tokens != 0:
+            raise ValueError("designs whose layers are listed keep their cache in the type of their parameters; their prompts go through in portions "
+                             "of max_prefill_tokens")
+        super()._init_cache_kind(kv_cache_dtype, prefill_chunk_tokens)
+
     def _init_sharing(self, tp: Any, prefix_caching: bool) -> None:
         if tp is not None and tp.size > 1:
             raise ValueError("tensor-parallel replicas are not built for this design")

@@ -48,6 +48,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     ap.add_argument("--max-seqs", type=int, default=256)
     ap.add_argument("--max-model-len", type=int, default=None)
     ap.add_argument("--max-prefill-tokens", type=int, default=16384)
+    ap.add_argument("--prefill-chunk-tokens", type=int, default=0, help="prompts go through in portions of at most so many tokens (0: whole)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"], help="fp8: keys and values in 8 bits")
     ap.add_argument("--kv-gb", type=float, default=None, help="memory for the KV cache (default: 60 %% of what is free)")
     ap.add_argument("--cuda-graphs", action="store_true", help="capture the decode step")
     args = ap.parse_args(argv)
@@ -64,7 +66,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     max_len = args.max_model_len or max(len(p) for p in prompts) + args.max_new_tokens + 1
     eng = load_engine(args.model, args.dtype, seed=args.seed, max_model_len=max_len, max_seqs=max(args.max_seqs, args.n),
                       max_prefill_tokens=args.max_prefill_tokens, use_cuda_graph=args.cuda_graphs,
-                      kv_memory_bytes=int(args.kv_gb * 2 ** 30) if args.kv_gb else None)
+                      kv_memory_bytes=int(args.kv_gb * 2 ** 30) if args.kv_gb else None, kv_cache_dtype=args.kv_cache_dtype,
+                      prefill_chunk_tokens=args.prefill_chunk_tokens)
     if args.logprobs:
         eng.enable_logprobs()
     for i, p in enumerate(prompts):

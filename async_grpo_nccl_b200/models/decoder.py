@@ -281,41 +281,66 @@ class NativeDecoder:
             save.update(x=x, h1=h1, rstd1=rstd1, qkv=qkv, attn=attn, lse=lse, x1=x1, h2=h2, rstd2=rstd2, gu=gu, act=act)
         return x2
 
-    def layer_fwd_suffix(self, i: int, x: torch.Tensor, batch: PackedBatch, sfx: torch.Tensor, pfx: torch.Tensor,
-                         pos_s: torch.Tensor, cos_t, sin_t, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
-                         pfx_blk: torch.Tensor, pfx_off: torch.Tensor) -> torch.Tensor:
+    def layer_fwd_suffix(self, i: int, x: torch.Tensor, batch: PackedBatch, sfx: torch.Tensor, pfx_slots: torch.Tensor,
+                         pos_s: torch.Tensor, cos_t, sin_t, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
         """Layer forward for a rollout prefill whose leading prompt tokens are already in the KV cache (prefix caching).
         ``x`` holds the rows of the tokens that still have to be computed (packed positions ``sfx`` of ``batch``, which
         describes the whole prompts). Projections and MLP run on those rows only; attention runs over the whole prompts
-        with the keys / values of the cached tokens (packed positions ``pfx``, cache block / offset ``pfx_blk`` /
-        ``pfx_off``) gathered from the cache. The query rows of cached tokens are zero and their outputs are dropped."""
+        with the keys / values of the cached tokens (``pfx_slots``: their cache slots at their packed positions, -1 at the others)
+        read back from the cache. The query rows of cached tokens are zero and their outputs are dropped."""
         cfg, C = self.cfg, self.C
-        Ts, T = x.shape[0], batch.T
+        T = batch.T
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+
+        def attend(qkv_s: torch.Tensor) -> torch.Tensor:
+            C.kv_cache_write(qkv_s, slots, k_cache, v_cache, Hq, Hkv, D, self.status, 0)
+            qkv = torch.zeros(T, cfg.qkv_dim, dtype=torch.bfloat16, device=x.device)
+            qkv.index_copy_(0, sfx, qkv_s)
+            C.kv_cache_read(k_cache, v_cache, pfx_slots, qkv, Hq, Hkv, D, self.status)
+            attn = self._new(T, cfg.q_dim)
+            lse = self._new(Hq, T, dtype=torch.float32)
+            C.attn_varlen_fwd(qkv, attn, lse, batch.tiles, Hq, Hkv, D, 1.0 / math.sqrt(D), self.status)
+            self.launches += 3
+            return attn.index_select(0, sfx)
+
+        return self._layer_fwd_around(i, x, pos_s, cos_t, sin_t, attend)
+
+    def layer_fwd_paged(self, i: int, x: torch.Tensor, pos: torch.Tensor, cos_t, sin_t, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], slots: torch.Tensor, tables: torch.Tensor,
+                        lens: torch.Tensor, starts: torch.Tensor) -> torch.Tensor:
+        """Layer forward for the newest tokens of some sequences: their keys and values go to ``slots`` of the paged cache (bf16, or 8 bits
+        with scale bytes), and their rows (``starts`` of every sequence's) attend over its pages (``tables``), of which ``lens`` tokens count."""
+        cfg, C = self.cfg, self.C
+        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+
+        def attend(qkv: torch.Tensor) -> torch.Tensor:
+            C.kv_cache_write(qkv, slots, k_cache, v_cache, Hq, Hkv, D, self.status, 0, k_scale, v_scale)
+            attn = self._new(qkv.shape[0], cfg.q_dim)
+            C.paged_chunk_attn(qkv, k_cache, v_cache, tables, lens, starts, attn, Hq, Hkv, D, 1.0 / math.sqrt(D), self.status, k_scale, v_scale)
+            self.launches += 3
+            return attn
+
+        return self._layer_fwd_around(i, x, pos, cos_t, sin_t, attend)
+
+    def _layer_fwd_around(self, i: int, x: torch.Tensor, pos: torch.Tensor, cos_t, sin_t, attend) -> torch.Tensor:
+        """A layer without what its backward pass needs; ``attend`` makes the attention output of the rows from their rotated q, k, v."""
+        cfg, C = self.cfg, self.C
+        T = x.shape[0]
         p = f"layers.{i}."
         self._enter_unit(i + 1, None)
-        h1 = self._new(Ts, cfg.hidden_size)
+        h1 = self._new(T, cfg.hidden_size)
         C.rmsnorm_fwd(x, self.w(p + "ln1"), h1, None, cfg.rms_norm_eps)
-        qkv_s = self._new(Ts, cfg.qkv_dim)
-        self._qkv(h1, p, qkv_s, pos_s, cos_t, sin_t)
-        C.kv_cache_write(qkv_s, slots, k_cache, v_cache, Hq, Hkv, D, self.status, 0)
-        qkv = torch.zeros(T, cfg.qkv_dim, dtype=torch.bfloat16, device=x.device)
-        qkv.index_copy_(0, sfx, qkv_s)
-        heads = qkv.view(T, Hq + 2 * Hkv, D)
-        heads[pfx, Hq:Hq + Hkv] = k_cache[pfx_blk, :, pfx_off]   # [cached tokens, Hkv, D]
-        heads[pfx, Hq + Hkv:] = v_cache[pfx_blk, :, pfx_off]
-        attn = self._new(T, cfg.q_dim)
-        lse = self._new(Hq, T, dtype=torch.float32)
-        C.attn_varlen_fwd(qkv, attn, lse, batch.tiles, Hq, Hkv, D, 1.0 / math.sqrt(D), self.status)
-        attn_s = attn.index_select(0, sfx)
-        x1 = self._new(Ts, cfg.hidden_size)
-        self._gemm(attn_s, self.w(p + "wo"), x1, residual=x)
-        h2 = self._new(Ts, cfg.hidden_size)
+        qkv = self._new(T, cfg.qkv_dim)
+        self._qkv(h1, p, qkv, pos, cos_t, sin_t)
+        attn = attend(qkv)
+        x1 = self._new(T, cfg.hidden_size)
+        self._gemm(attn, self.w(p + "wo"), x1, residual=x)
+        h2 = self._new(T, cfg.hidden_size)
         C.rmsnorm_fwd(x1, self.w(p + "ln2"), h2, None, cfg.rms_norm_eps)
         _, act = self._mlp_in(h2, self.w(p + "wgu"), False)
-        x2 = self._new(Ts, cfg.hidden_size)
+        x2 = self._new(T, cfg.hidden_size)
         self._gemm(act, self.w(p + "wd"), x2, residual=x1)
-        self.launches += 4
+        self.launches += 2
         return x2
 
     def _layer_bwd(self, i: int, dx: torch.Tensor, s: dict, batch: PackedBatch, cos_t, sin_t, sink: GradSink):

@@ -60,3 +60,14 @@ def test_tensors_on_the_host_are_refused(op):
             C.kv_cache_read(k, k, i[:2], rows, 1, 1, 64, None, s, s)
         else:
             C.paged_chunk_attn(rows, k, k, i[:2, None], i, i, torch.empty(2, 64, dtype=torch.bfloat16), 1, 1, 64, 0.1, None, s, s)
+
+
+def test_configuration_keys():
+    from async_grpo_nccl_b200.config import make_config
+
+    assert make_config({"kv_cache_dtype": "fp8", "prefill_chunk_tokens": 512}).kv_cache_dtype == "fp8"
+    for bad in ({"kv_cache_dtype": "int8"}, {"prefill_chunk_tokens": -1},
+                {"kv_cache_dtype": "fp8", "generation_tp_size": 2, "num_generation_gpu_workers": 2},
+                {"prefill_chunk_tokens": 64, "generation_tp_size": 2, "num_generation_gpu_workers": 2}):
+        with pytest.raises(ValueError):
+            make_config(bad)
