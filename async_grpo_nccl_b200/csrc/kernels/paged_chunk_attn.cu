@@ -31,6 +31,7 @@ constexpr int kBN = 128;  // keys a tile
 template <int D>
 constexpr int kGroupBytes = D / 64 * 1024;
 
+constexpr int kExtra = 1;      // a unit's beginning and end, in tiles
 constexpr int kSeqRoom = 128;  // sequences that a CTA has at hand
 
 template <int D, bool k8>
@@ -122,8 +123,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   }
   pdl_wait();
   pdl_launch();
-  measure_line<S::kThreads, kBN>(p, reinterpret_cast<int*>(ring));
-  const Share share = find_share<kBN, 1>(p, reinterpret_cast<const int*>(ring), blockIdx.x, gridDim.x);
+  measure_line<S::kThreads, kBN, kExtra>(p, reinterpret_cast<int*>(ring));
+  const Share share = find_share<kBN, kExtra, 1>(p, reinterpret_cast<const int*>(ring), blockIdx.x, gridDim.x);
   const SeqCache near = {reinterpret_cast<int*>(smem + S::kSeqOff), share.b, kSeqRoom};
   near.fill(p);
   fence_proxy_async_smem();  // the line lies where the ring's copies go next
@@ -131,7 +132,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walk<kBN> w;  // every warp walks by itself
+  Walk<kBN, kExtra> w;  // every warp walks by itself
   w.start(p, share, near);
 
   if (warp == S::kLoadWarp) {
@@ -294,7 +295,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     uint8_t* raw = smem + S::kRawOff + tid * 16;
     uint8_t* raw_scale = smem + S::kScaleOff + cw * 32;
     const int sub = lane >> 2;                   // row of the eight
-    Walk<kBN> a = w;                             // the copies' walk
+    Walk<kBN, kExtra> a = w;                             // the copies' walk
     int a_j = a.j0, a_v = 0, n_copy = 0, page = 0;
     // Blocks of the table that hold this warp's rows of the tile: lane i < 4 those from row 32 i + 8 cw on.
     const auto pages = [&] {
@@ -401,7 +402,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     bool ok = true;
     if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     int flat = share.before;
-    for (; w.more() && ok; flat += w.j1 - w.j0, w.next(p)) {
+    for (; w.more() && ok; flat += w.length(), w.next(p)) {
       const int rows = max(min(p.tile_tokens, w.tokens(p) - t * p.tile_tokens), 0) * p.G;  // of this tile
       const bool busy = quarter * 32 < rows;                                               // the warp has rows
       const int end = w.end_of(p, t);

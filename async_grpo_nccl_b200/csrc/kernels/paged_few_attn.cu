@@ -32,6 +32,7 @@ namespace agrpo {
 namespace {
 
 constexpr int kKeys = 16;
+constexpr int kExtra = 4;          // a unit's beginning and end, in tiles
 constexpr int kSeqRoom = 128;      // sequences that a CTA has at hand
 constexpr float kNone = -3.0e38f;  // maximum of nothing: finite, so that a difference with it is a number
 
@@ -105,16 +106,16 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
   if (threadIdx.x <= kW) jobs[threadIdx.x].tokens = 0;
   pdl_wait();
   pdl_launch();
-  measure_line<kW * 32, kKeys>(p, line);
+  measure_line<kW * 32, kKeys, kExtra>(p, line);
   const int worker = blockIdx.x * kW + warp;
-  const Share share = find_share<kKeys, 2>(p, line, worker, gridDim.x * kW);
+  const Share share = find_share<kKeys, kExtra, 2>(p, line, worker, gridDim.x * kW);
   __shared__ int seqs[3 * kSeqRoom], first_seq;
   if (threadIdx.x == 0) first_seq = share.b;
   __syncthreads();  // the line is read, parts come there
   const SeqCache near = {seqs, first_seq, kSeqRoom};
   near.fill(p);
   __syncthreads();
-  Walk<kKeys> w;
+  Walk<kKeys, kExtra> w;
   w.start(p, share, near);
   if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
 
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
   const auto* vs_lane = p.c.v_scale + 2 * t;
   int flat = share.before;
 
-  for (; w.more(); flat += w.j1 - w.j0, w.next(p)) {
+  for (; w.more(); flat += w.length(), w.next(p)) {
     const int keys = unit_keys(p, w.s, w.qb), rows = w.tokens(p) * G;
     const long long row0 = w.s.row0 + w.qb * p.tokens;
     const int first_pos = w.s.len - w.s.n + w.qb * p.tokens;  // position of the unit's first row: it sees the keys up to there
