@@ -40,10 +40,10 @@ struct Shape {
   static constexpr int kSlotBytes = kBN * D * 2;              // a tile of K or V in bf16
   static constexpr int kQBytes = 2 * 128 * D * 2;
   static constexpr int kSlots = k8 ? 4 : 5;
-  static constexpr int kRaw = k8 ? 2 : 0;                     // tiles of codes under way
+  static constexpr int kRaw = k8 ? 2 : 0;                     // tiles of codes under way: one of K, one of V
   static constexpr int kMmaWarp = 8, kLoadWarp = 9;
-  static constexpr int kConvWarp = 12;                        // 8 bits: four warpgroups, registers dealt out anew; warps 10 and 11 do nothing
-  static constexpr int kThreads = k8 ? 512 : 320;
+  static constexpr int kConvWarp = 12;                        // 8 bits: five warpgroups, registers dealt out anew; warps 10 and 11 do nothing
+  static constexpr int kThreads = k8 ? 640 : 320;
   static constexpr int kRingOff = kQBytes;
   static constexpr int kRawOff = kRingOff + kSlots * kSlotBytes;
   static constexpr int kScaleOff = kRawOff + kRaw * kBN * D;
@@ -61,12 +61,8 @@ __device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool on)
 __device__ __forceinline__ void cp_async_4(void* dst, const void* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// 8 bits: registers of the warpgroups, 128 x (168 + 168 + 72 + 104) = the launch's 512 x 128.
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// 8 bits: registers of the warpgroups, 128 x (144 + 144 + 64 + 64 + 64) = the launch's 640 x 96.
 template <bool kOn, int kLeft>
 __device__ __forceinline__ void give_registers() {
   if (kOn) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeft));
@@ -136,7 +132,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   w.start(p, share, near);
 
   if (warp == S::kLoadWarp) {
-    give_registers<k8, 72>();
+    give_registers<k8, 64>();
     // ---------------------------------------------------------------- copies
     // The first tile of a piece goes ahead of its Q, which has to wait for the last products with the one before. (8 bits: Q alone comes from here.)
     int item = 0, n_q = 0;
@@ -194,7 +190,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
     }
   } else if (warp == S::kMmaWarp) {
-    give_registers<k8, 72>();
+    give_registers<k8, 64>();
     // ---------------------------------------------------------------- products
     const uint32_t aQ = smem_u32(smem), aRing = smem_u32(ring);
     int tile = 0, n_q = 0;          // tiles and pieces so far
@@ -284,34 +280,34 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
     }
   } else if (k8 && warp >= S::kConvWarp) {
-    give_registers<k8, 104>();
+    give_registers<k8, 64>();
     // ---------------------------------------------------------------- 8 bits to bf16
     // 16 codes a thread and step. A warp has 8 rows of every 32 (two steps for them if D = 128): eight lanes take four pieces of a row and the other
     // four of the next one, so that their 16-byte writes fall into eight different bank groups. A thread copies the pieces that it will turn into bf16
     // itself, so nobody waits for anybody else's copies. (Bulk copies of pages of 16 tokens, 2 KB, took 54 cycles each to issue.)
-    const int cw = warp - S::kConvWarp, tid = cw * 32 + lane;
-    constexpr int kRaw = S::kRaw > 0 ? S::kRaw : 1;
+    const int v = (warp - S::kConvWarp) >> 2, cw = (warp - S::kConvWarp) & 3;  // four warps for K, four for V, with slots of their own
     constexpr int kPerRows = D / 64;             // steps for the same rows
-    uint8_t* raw = smem + S::kRawOff + tid * 16;
-    uint8_t* raw_scale = smem + S::kScaleOff + cw * 32;
+    uint8_t* raw = smem + S::kRawOff + v * (kBN * D) + (cw * 32 + lane) * 16;
+    uint8_t* raw_scale = smem + S::kScaleOff + v * kBN + cw * 32;
+    const auto* codes = static_cast<const uint8_t*>(v ? p.c.v : p.c.k);
+    const auto* scales = v ? p.c.v_scale : p.c.k_scale;
     const int sub = lane >> 2;                   // row of the eight
     Walk<kBN, kExtra> a = w;                             // the copies' walk
-    int a_j = a.j0, a_v = 0, n_copy = 0, page = 0;
+    int a_j = a.j0, page = 0;
     // Blocks of the table that hold this warp's rows of the tile: lane i < 4 those from row 32 i + 8 cw on.
     const auto pages = [&] {
       if (!a.more()) return;
       const int key = a_j * kBN + (lane & 3) * 32 + cw * 8;
       page = key < unit_keys(p, a.s, a.qb) ? p.a.block_tables[a.b * p.a.table_pitch + key / p.c.block_size] : 0;
-      if (page < 0 || page >= p.c.num_blocks) {
-        report_status(status, kStatusBadIndex);
-        page = 0;
-      }
     };
     const auto copy = [&] {
       if (a.more()) {
-        const int slot = n_copy % kRaw, bs = p.c.block_size;
+        if (page < 0 || page >= p.c.num_blocks) {
+          report_status(status, kStatusBadIndex);
+          page = 0;
+        }
+        const int bs = p.c.block_size;
         const int valid = unit_keys(p, a.s, a.qb) - a_j * kBN;
-        const auto* codes = static_cast<const uint8_t*>(a_v ? p.c.v : p.c.k);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int r = q * 32 + cw * 8 + sub;
@@ -319,79 +315,70 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
           for (int h = 0; h < kPerRows; ++h) {
             const int piece = D == 128 ? (lane & 3) + 4 * ((sub & 1) ^ h) : lane & 3;
-            cp_async_16(raw + slot * (kBN * D) + (q * kPerRows + h) * 2048, codes + row * D + piece * 16, r < valid);
+            cp_async_16(raw + (q * kPerRows + h) * 2048, codes + row * D + piece * 16, r < valid);
           }
         }
         // the factors' bytes: four rows a lane
         const int pq = __shfl_sync(0xffffffffu, page, lane >> 1 & 3), r = (lane >> 1 & 3) * 32 + cw * 8 + (lane & 1) * 4;
         if (lane < 8) {
           const long long row = (static_cast<long long>(pq) * p.c.Hkv + a.kvh) * bs + ((a_j * kBN + r) & (bs - 1));
-          cp_async_4(raw_scale + slot * kBN + lane * 4, (a_v ? p.c.v_scale : p.c.k_scale) + row, r < valid);
+          cp_async_4(raw_scale + lane * 4, scales + row, r < valid);
         }
-        ++n_copy;
-        a_v ^= 1;
-        if (a_v == 0) {
-          if (++a_j == a.j1) {
-            a.next(p);
-            a_j = a.j0;
-          }
-          pages();
+        if (++a_j == a.j1) {
+          a.next(p);
+          a_j = a.j0;
         }
+        pages();
       }
-      cp_async_commit();  // also where nothing is left, so that the waits below name the same tile
     };
     pages();
-#pragma unroll 1
-    for (int i = 0; i < kRaw; ++i) copy();
-    int item = 0;
+    copy();
+    int item = v;
     bool ok = true;
     for (; w.more() && ok; w.next(p)) {
-      for (int j = w.j0; j < w.j1 && ok; ++j) {
-        for (int v = 0; v < 2; ++v, ++item) {
-          const int slot = item % S::kSlots, round = item / S::kSlots, mine = item % kRaw;
-          cp_async_wait<kRaw - 1>();
-          __syncwarp();
-          // of row 32 (lane / 8) + 8 cw + lane % 8. Behind the last key the codes are zero, and the factor has to be a number
-          const int left = unit_keys(p, w.s, w.qb) - j * kBN - cw * 8;
-          const Kv8Scale s = kv8_scale((lane >> 3) * 32 + (lane & 7) < left ? raw_scale[mine * kBN + lane] : 0);
-          const bool twice = __any_sync(0xffffffffu, s.twice);         // some value above 448 * 2^7
-          if (round > 0 && !mbar_wait(empty + slot, (round - 1) & 1)) {
-            report_status(status, kStatusWaitEmptyTimeout);
-            ok = false;
-            break;
-          }
-          const uint8_t* src = raw + mine * (kBN * D);
-          uint8_t* dst = ring + slot * S::kSlotBytes + cw * kGroupBytes<D> + sub * 128;
-          const auto convert = [&](auto both) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              Kv8Scale f;
-              f.first = __shfl_sync(0xffffffffu, s.first, q * 8 + sub);
-              f.second = decltype(both)::value ? __shfl_sync(0xffffffffu, s.second, q * 8 + sub) : 0u;
-              f.twice = decltype(both)::value ? __shfl_sync(0xffffffffu, static_cast<int>(s.twice), q * 8 + sub) != 0 : false;
-#pragma unroll
-              for (int h = 0; h < kPerRows; ++h) {
-                const uint4 x = *reinterpret_cast<const uint4*>(src + (q * kPerRows + h) * 2048);
-                const uint2 e = kv8_decode4(x.x, f), g = kv8_decode4(x.y, f), y = kv8_decode4(x.z, f), z = kv8_decode4(x.w, f);
-                uint8_t* row = dst + q * 4 * kGroupBytes<D> + (D == 128 ? ((sub & 1) ^ h) * 1024 : 0);
-                const int ch = (lane & 3) * 2;
-                *reinterpret_cast<uint4*>(row + ((ch ^ sub) << 4)) = make_uint4(e.x, e.y, g.x, g.y);
-                *reinterpret_cast<uint4*>(row + (((ch + 1) ^ sub) << 4)) = make_uint4(y.x, y.y, z.x, z.y);
-              }
-            }
-          };
-          if (twice) convert(std::true_type{});
-          else convert(std::false_type{});
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + slot);
-          copy();
+      for (int j = w.j0; j < w.j1; ++j, item += 2) {
+        const int slot = item % S::kSlots, round = item / S::kSlots;
+        cp_async_wait_all();
+        __syncwarp();
+        // of row 32 (lane / 8) + 8 cw + lane % 8. Behind the last key the codes are zero, and the factor has to be a number
+        const int left = unit_keys(p, w.s, w.qb) - j * kBN - cw * 8;
+        const Kv8Scale s = kv8_scale((lane >> 3) * 32 + (lane & 7) < left ? raw_scale[lane] : 0);
+        const bool twice = __any_sync(0xffffffffu, s.twice);         // some value above 448 * 2^7
+        if (round > 0 && !mbar_wait(empty + slot, (round - 1) & 1)) {
+          report_status(status, kStatusWaitEmptyTimeout);
+          ok = false;
+          break;
         }
+        uint8_t* dst = ring + slot * S::kSlotBytes + cw * kGroupBytes<D> + sub * 128;
+        const auto convert = [&](auto both) {
+#pragma unroll 2
+          for (int q = 0; q < 4; ++q) {
+            Kv8Scale f;
+            f.first = __shfl_sync(0xffffffffu, s.first, q * 8 + sub);
+            f.second = decltype(both)::value ? __shfl_sync(0xffffffffu, s.second, q * 8 + sub) : 0u;
+            f.twice = decltype(both)::value ? __shfl_sync(0xffffffffu, static_cast<int>(s.twice), q * 8 + sub) != 0 : false;
+#pragma unroll
+            for (int h = 0; h < kPerRows; ++h) {
+              const uint4 x = *reinterpret_cast<const uint4*>(raw + (q * kPerRows + h) * 2048);
+              const uint2 e = kv8_decode4(x.x, f), g = kv8_decode4(x.y, f), y = kv8_decode4(x.z, f), z = kv8_decode4(x.w, f);
+              uint8_t* row = dst + q * 4 * kGroupBytes<D> + (D == 128 ? ((sub & 1) ^ h) * 1024 : 0);
+              const int ch = (lane & 3) * 2;
+              *reinterpret_cast<uint4*>(row + ((ch ^ sub) << 4)) = make_uint4(e.x, e.y, g.x, g.y);
+              *reinterpret_cast<uint4*>(row + (((ch + 1) ^ sub) << 4)) = make_uint4(y.x, y.y, z.x, z.y);
+            }
+          }
+        };
+        if (twice) convert(std::true_type{});
+        else convert(std::false_type{});
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + slot);
+        copy();
       }
     }
-    cp_async_wait<0>();
+    cp_async_wait_all();
   } else if (warp < S::kMmaWarp) {
-    take_registers<k8, 168>();
+    take_registers<k8, 144>();
     // ---------------------------------------------------------------- softmax, results
     const int t = warp >> 2, quarter = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -579,7 +566,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         p.desc[blockIdx.x] = make_int4(w.s.row0 + w.qb * p.tokens, w.tokens(p), w.kvh, w.last_worker(share, flat));
     }
   } else {
-    give_registers<k8, 72>();
+    give_registers<k8, 64>();
   }
 
   tc_fence_before();

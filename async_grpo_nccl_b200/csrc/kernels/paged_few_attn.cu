@@ -9,10 +9,11 @@
 // Which dim of a head a lane holds is free as long as Q agrees (in S) or the result is put back (in O): a lane has consecutive ones, so that its loads are 16 bytes
 // and 4 (K) or 8 (V) lanes read a whole 64 or 128 bytes.
 //
-// 8 bits: the products are fp16, since one instruction turns two codes into fp16, exactly, and bf16 would take five (moves, masks, a product): 310 -> XXX us for 128
-// rows over 1000 - 8000 tokens. fp16's exponents are few, so powers of two are kept apart: a row of Q is scaled to a maximum of 2^14 .. 2^15 (28 binades down to
-// fp16's subnormals are exact), a key's own power goes into the fp32 factor of its scores, probabilities are held times 2^7 (at most 2^15; below 2^-31 they vanish),
-// and O is held relative to a power of two F that the values of 16 keys may differ from by 2^14; where they differ by more, those 16 keys take the bf16 products.
+// 8 bits: the products are fp16, since one instruction turns two codes into fp16, exactly, and bf16 would take five (moves, masks, a product): 312 -> 240 us for 128
+// rows of 40 heads over 1000 - 8000 tokens. fp16's exponents are few, so powers of two are kept apart: a row of Q is scaled to a maximum of 2^14 .. 2^15 (28 binades
+// down to fp16's subnormals are exact), a key's own power goes into the fp32 factor of its scores, probabilities are held times 2^13 (at most 2^15; below 2^-37 they
+// vanish), and O is held relative to a power of two F that the values of 16 keys may be up to 2^14 below; where they are further below, and after F has grown by
+// more than 2^14 (a vanished probability could then have counted), 16 keys take the bf16 products.
 //
 // mma.sync and not tcgen05: at 8 to 16 rows the products are a hundredth of what tcgen05 could do, and its hand-overs (tile in shared memory, barrier, product,
 // barrier, scores from tensor memory, probabilities back, barrier) cost more than the keys' bytes: those rows took 490 us that way.
@@ -53,22 +54,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-// Two e4m3 codes (the lower or the upper half of a word) as fp16.
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w, bool upper) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(upper ? w >> 16 : w));
-  return d;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
 __device__ __forceinline__ float power(int byte) { return __uint_as_float(static_cast<uint32_t>(byte) << 23); }  // 2^(byte - 127)
 
 // kN: query rows / 8 of a unit.
@@ -94,7 +79,8 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
   constexpr int kKW = k8 ? D / 16 : D / 8;  // words of a key's dims that a lane holds (K: D / 4 dims)
   constexpr int kVW = k8 ? D / 32 : D / 16; // likewise of V (D / 8 dims)
   constexpr int kRow = k8 ? D : 2 * D;      // bytes of a key
-  constexpr float kLift = k8 ? 7.f : 0.f;   // probabilities are held times 2^kLift
+  constexpr float kLift = k8 ? 13.f : 0.f;  // probabilities are held times 2^kLift ...
+  constexpr float kSlack = k8 ? 2.f : 8.f;  // ... and relative to a maximum that may have grown by this many binades since
 
   extern __shared__ __align__(16) uint8_t shared[];
   float* part_o = reinterpret_cast<float*>(shared);
@@ -259,7 +245,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
-    int v_pow = 0;                 // 8 bits: F + 127; O is held in 2^F
+    int v_pow = 0, v_first = 0;    // 8 bits: F + 127, at first; O is held in 2^F
 
     for (int j = w.j0; j < w.j1; ++j) {
       // ---- S^T: 16 keys x 8 kN rows
@@ -287,8 +273,8 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
       // the keys' own factors
       float key_pow[2] = {1.f, 1.f};
       if (k8) {
-        key_pow[0] = power(k_byte[0]);  // 255: infinity, and 0 * infinity is the NaN that is wanted
-        key_pow[1] = power(k_byte[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) key_pow[h] = k_byte[h] == kKv8NanByte ? __uint_as_float(0x7fffffffu) : power(k_byte[h]);
       }
       const bool more = j + 1 < w.j1;
       const int left = keys - (j + 1) * kKeys;
@@ -319,7 +305,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
         for (int i = 0; i < 4; ++i) z[n][i] = s[n][i] - m[n][i & 1];
         top = max3(top, max3(z[n][0], z[n][1], z[n][2]), z[n][3]);
       }
-      if (__any_sync(0xffffffffu, top > 8.f + kLift)) {  // some maximum has grown by more than 2^8
+      if (__any_sync(0xffffffffu, top > kSlack + kLift)) {  // some maximum has grown by more than that
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -369,6 +355,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
           if (most > v_pow) {
             const float down = v_pow == 0 ? 0.f : power(max(127 + v_pow - most, 0));
             v_pow = most;
+            if (v_first == 0) v_first = most;
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -383,7 +370,7 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
           }
           good = fits();
         }
-        if (good) {
+        if (good && v_pow <= v_first + 14) {
           const uint32_t c = static_cast<uint32_t>(15 - v_pow) * 0x10001u;
           const uint32_t f16[2] = {(f[0] + c) << 10, (f[1] + c) << 10};
 #pragma unroll

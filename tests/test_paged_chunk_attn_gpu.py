@@ -109,6 +109,86 @@ def test_large_logits(n, eight):
     c.check()
 
 
+@pytest.mark.parametrize("seqs", [[(1, 900)] * 3, [(60, 900), (200, 500)]])
+@pytest.mark.parametrize("which,spread", [(0, 8), (0, 60), (1, 8), (1, 20), (1, 60), (2, 30)])
+def test_keys_and_values_of_very_different_sizes(seqs, which, spread):
+    """8 bits: every vector with a power of its own, up to 2^spread apart (0: keys, 1: values, 2: both); a third of the values' vectors is zero."""
+    c = Case(seqs, 12, 2, 128, 16, True, seed=spread)
+    g = torch.Generator(device=DEV).manual_seed(which)
+    for i in range(2):
+        if which not in (i, 2):
+            continue
+        held = c.scales[i] != 255
+        e = torch.randint(-spread, 1, held.shape, device=DEV, generator=g)
+        x = torch.randn(c.kv[i].shape, device=DEV, generator=g).double() * torch.exp2(e.double())[..., None]
+        if i == 1:
+            x[torch.rand(held.shape, device=DEV, generator=g) < 0.33] = 0
+        codes, s = R.kv8_quantise(x.bfloat16().float())
+        c.values[i] = R.kv8_values(codes, s)
+        codes.view(torch.uint8).masked_fill_(~held[..., None], 0x7f)
+        c.kv[i], c.scales[i] = codes, s.masked_fill(~held, 255)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("seqs", [[(1, 900)] * 3, [(60, 900), (200, 500)]])
+def test_values_that_grow_along_the_sequence(seqs):
+    """8 bits: later pages hold values up to 2^40 larger, whose probabilities are small."""
+    c = Case(seqs, 12, 2, 128, 16, True, seed=9)
+    held = c.scales[1] != 255
+    where = torch.zeros(held.shape[0], device=DEV)
+    for b, (_, total) in enumerate(seqs):
+        n = -(-total // 16)
+        where[c.table[b, :n].long()] = torch.arange(n, device=DEV) * 40.0 / n
+    x = torch.randn(c.kv[1].shape, device=DEV) * torch.exp2(where.floor())[:, None, None, None]
+    codes, s = R.kv8_quantise(x)
+    c.values[1] = R.kv8_values(codes, s)
+    c.kv[1], c.scales[1] = codes, s.masked_fill(~held, 255)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 300)], [(70, 300), (70, 300)]])
+def test_a_nan_stays_with_the_rows_that_see_it(seqs, eight):
+    """A key or a value that is NaN makes its own sequence's rows NaN, those that see it and no other sequence's."""
+    for i in range(2):
+        c = Case(seqs, 12, 2, 128, 16, eight, seed=11)
+        page, off = int(c.table[0, 3]), 5   # token 53 of sequence 0, kv head 1
+        if eight:
+            c.scales[i][page, 1, off] = 255
+        else:
+            c.kv[i][page, 1, off, 7] = math.nan
+        c.call()
+        n = seqs[0][0]
+        heads = c.out.view(-1, 2, 6 * 128)
+        assert bool(heads[n:].isfinite().all()) and bool(heads[:n, 0].isfinite().all())
+        bad = heads[:n, 1].view(n, 6, 128)
+        assert bool(bad.isnan().all()) if i == 0 or eight else bool(bad[..., 7].isnan().all()) and bool(bad[..., :7].isfinite().all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_queries_of_any_size(eight):
+    """Rows of Q from subnormal to 2^60, one of zeros: with keys as small as the queries are large, logits stay moderate."""
+    for n in (1, 50):
+        c = Case([(n, 300)] * 2, 12, 2, 128, 16, eight, seed=12)
+        e = torch.tensor([-100.0, -30.0, 0.0, 1.0], device=DEV)[torch.arange(c.rows.shape[0], device=DEV) % 4]
+        c.rows = (c.rows.double() * torch.exp2(e.double())[:, None]).bfloat16()
+        c.rows[0] = 0
+        c.call()
+        c.check()
+        c.rows = (c.rows.float() * 2.0 ** 59).bfloat16()
+        small = c.values[0].double() * 2.0 ** -59
+        if eight:
+            codes, s = R.kv8_quantise(small.float())
+            c.kv[0], c.scales[0], c.values[0] = codes, s, R.kv8_values(codes, s)
+        else:
+            c.kv[0] = c.values[0] = small.bfloat16()
+        c.out.fill_(7)
+        c.call()
+        c.check()
+
+
 def test_a_sequence_does_not_depend_on_where_its_pages_are():
     a = Case([(5, 700), (300, 900)], 12, 2, 128, 16, False, seed=1)
     a.call()
