@@ -685,6 +685,7 @@ void kv_cache_write(const Tensor& qkv, const Tensor& slots, Tensor& k_cache, Ten
     cache_args::rows(qkv, (Hq + 2 * Hkv) * D, op, "qkv");
     const agrpo::PagedCache c = cache_args::cache(k_cache, v_cache, k_scale, v_scale, qkv.device(), D, op);
     TORCH_CHECK(c.Hkv + kv_head0 <= Hkv, op, ": cache [blocks, kv heads of this rank, bs, D]");
+    cache_args::vectors(qkv.size(0), c.Hkv, op);
     cache_args::ints(slots, qkv.device(), 0, op, "slots");
     TORCH_CHECK(slots.numel() == qkv.size(0), op, ": a slot for each row");
     cache_args::status_word(status, qkv.device(), op);

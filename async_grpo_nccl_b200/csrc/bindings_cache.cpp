@@ -22,6 +22,7 @@ void kv_cache_read(const Tensor& k_cache, const Tensor& v_cache, const Tensor& s
   TORCH_CHECK(c.Hkv == Hkv, op, ": cache of ", std::to_string(Hkv), " kv heads");
   ints(slots, qkv.device(), 0, op, "slots");
   TORCH_CHECK(slots.numel() == qkv.size(0), op, ": a slot for each row");
+  vectors(qkv.size(0), c.Hkv, op);
   status_word(status, qkv.device(), op);
   const c10::cuda::CUDAGuard guard(qkv.device());
   agrpo::launch_kv_cache_read(c, slots.data_ptr<int>(), qkv.data_ptr(), qkv.stride(0), (int)(Hq * D), (int)((Hq + Hkv) * D), (int)qkv.size(0),

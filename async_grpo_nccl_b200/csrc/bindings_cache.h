@@ -34,6 +34,8 @@ inline void written_rows(const Tensor& t, int64_t cols, const char* op, const ch
   rows(t, cols, op, name);
   TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= cols, op, ": ", name, " rows overlap");
 }
+// the kernels count the K and V vectors of a call in 31 bits
+inline void vectors(int64_t rows, int64_t heads, const char* op) { TORCH_CHECK(rows * 2 * heads < (int64_t(1) << 31), op, ": too many rows"); }
 // k and v [blocks, heads, block size, D] of one type: bf16, or e4m3 with scale bytes [blocks, heads, block size]
 inline agrpo::PagedCache cache(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs, const torch::Device& dev, int64_t D, const char* op) {
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.is_contiguous() && v.is_contiguous() && k.size(3) == D, op,

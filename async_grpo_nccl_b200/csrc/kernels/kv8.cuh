@@ -32,16 +32,17 @@ __device__ __forceinline__ uint32_t kv8_top(const uint4& v) {
 __device__ __forceinline__ uint2 kv8_encode(const uint4& v, int byte) {
   if (byte == kKv8NanByte) return make_uint2(0u, 0u);
   const float inv = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
-  const float lim = byte >= kKv8TopByte ? 240.f : 448.f;
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float2 f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);  // at most 448
+  if (byte >= kKv8TopByte) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(fminf(fmaxf(f[i].x, -240.f), 240.f), fminf(fmaxf(f[i].y, -240.f), 240.f));
+  }
   uint32_t half[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 f = make_float2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
-    f.x = fminf(fmaxf(f.x, -lim), lim);
-    f.y = fminf(fmaxf(f.y, -lim), lim);
-    half[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-  }
+  for (int i = 0; i < 4; ++i) half[i] = __nv_cvt_float2_to_fp8x2(f[i], __NV_SATFINITE, __NV_E4M3);
   return make_uint2(half[0] | (half[1] << 16), half[2] | (half[3] << 16));
 }
 
@@ -80,6 +81,24 @@ __device__ __forceinline__ uint2 kv8_decode4(uint32_t codes, const Kv8Scale& s) 
     hi = mul_bf16x2(hi, s.second);
   }
   return make_uint2(lo, hi);
+}
+
+// ---- fp16, for the products over an 8-bit cache
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// Two e4m3 codes (the lower or the upper half of a word) as fp16.
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w, bool upper) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(upper ? w >> 16 : w));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
 }  // namespace agrpo

@@ -1,5 +1,6 @@
 // KV cache in 8 bits: written from the rows of a prefill, written by a decode step with its rotation, read back into rows.
-// All three move bytes: a vector of D bf16 values is 2 D bytes on one side and D + 1 on the other.
+// All three move bytes: a vector of D bf16 values is 2 D bytes on one side and D + 1 on the other. 16384 rows of 8 kv heads of 128 written and read back: 200 MB in
+// 46 us (4.4 TB/s), 21 and 20 us by themselves; what is left above the 31 us of memory is the address arithmetic, a third of the instructions.
 #include <cuda_bf16.h>
 
 #include "../common/ptx.cuh"
@@ -22,61 +23,74 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
   return v;
 }
 
-// D / 8 lanes a vector, 16 bytes of bf16 each.
+// Where vector `vec` of a call lies: row t, heads [0, Hkv) of K, then of V. 32-bit arithmetic: with 64-bit divisions the kernels were bound by them (16384 rows of 8 kv
+// heads, written and read back: 61 us; more than one vector a group of lanes took longer).
+struct Vector {
+  unsigned t;
+  int head;
+  bool is_v;
+};
+__device__ __forceinline__ Vector vector_at(unsigned vec, int Hkv) {
+  Vector x;
+  x.t = vec / (2u * Hkv);
+  const int which = static_cast<int>(vec - x.t * (2u * Hkv));
+  x.is_v = which >= Hkv;
+  x.head = x.is_v ? which - Hkv : which;
+  return x;
+}
+// Its place in the cache, counted in vectors; -1: none. `first` lane reports a slot behind the cache.
+__device__ __forceinline__ long long place_of(const PagedCache& c, int slot, int head, bool first, int* status) {
+  if (slot < 0) return -1;
+  const int block = slot / c.block_size;
+  if (block >= c.num_blocks) {
+    if (first) report_status(status, kStatusBadIndex);
+    return -1;
+  }
+  return (static_cast<long long>(block) * c.Hkv + head) * c.block_size + (slot - block * c.block_size);
+}
+
+// D / 16 lanes a vector, 32 bytes of bf16 each: what is done once a lane (where the vector lies, its power) takes as many instructions as 16 values do.
 template <int D>
 __global__ void __launch_bounds__(kThreads)
 kv8_write_kernel(const __nv_bfloat16* __restrict__ qkv, long long pitch, int k_col0, int v_col0, const int* __restrict__ slots, PagedCache c,
-                 long long vectors, int* status) {
-  constexpr int kLanes = D / 8;
+                 unsigned vectors, int* status) {
+  constexpr int kLanes = D / 16;
   const int lane = threadIdx.x % kLanes;
-  const long long vec = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-  const int per_row = 2 * c.Hkv;
-  const bool on = vec < vectors;
-  const long long t = on ? vec / per_row : 0;
-  const int which = on ? static_cast<int>(vec - t * per_row) : 0;
-  const bool is_v = which >= c.Hkv;
-  const int h = is_v ? which - c.Hkv : which;
-  const int slot = on ? slots[t] : -1;
-  const bool bad = slot >= 0 && slot / c.block_size >= c.num_blocks;
-  if (bad && lane == 0) report_status(status, kStatusBadIndex);
-  const bool write = slot >= 0 && !bad;
-  uint4 x = make_uint4(0u, 0u, 0u, 0u);
-  if (write) x = *reinterpret_cast<const uint4*>(qkv + t * pitch + (is_v ? v_col0 : k_col0) + h * D + lane * 8);
-  const int byte = kv8_scale_byte(group_max<kLanes>(kv8_top(x)));
-  if (!write) return;
-  const long long at = (static_cast<long long>(slot / c.block_size) * c.Hkv + h) * c.block_size + slot % c.block_size;
-  uint8_t* codes = static_cast<uint8_t*>(is_v ? c.v : c.k) + at * D + lane * 8;
-  *reinterpret_cast<uint2*>(codes) = kv8_encode(x, byte);
-  if (lane == 0) (is_v ? c.v_scale : c.k_scale)[at] = static_cast<uint8_t>(byte);
+  const unsigned vec = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+  long long at = -1;
+  const Vector w = vector_at(min(vec, vectors - 1), c.Hkv);
+  if (vec < vectors) at = place_of(c, slots[w.t], w.head, lane == 0, status);
+  if (at >= 0) {
+    const auto* src = reinterpret_cast<const uint4*>(qkv + w.t * pitch + (w.is_v ? v_col0 : k_col0) + w.head * D + lane * 16);
+    x = src[0];
+    y = src[1];
+  }
+  const int byte = kv8_scale_byte(group_max<kLanes>(max(kv8_top(x), kv8_top(y))));
+  if (at < 0) return;
+  const uint2 a = kv8_encode(x, byte), b = kv8_encode(y, byte);
+  *reinterpret_cast<uint4*>(static_cast<uint8_t*>(w.is_v ? c.v : c.k) + at * D + lane * 16) = make_uint4(a.x, a.y, b.x, b.y);
+  if (lane == 0) (w.is_v ? c.v_scale : c.k_scale)[at] = static_cast<uint8_t>(byte);
 }
 
 // D / 16 lanes a vector: 16 codes (or 32 bytes of bf16) each.
 template <int D, bool k8>
 __global__ void __launch_bounds__(kThreads)
 kv_cache_read_kernel(PagedCache c, const int* __restrict__ slots, __nv_bfloat16* __restrict__ qkv, long long pitch, int k_col0, int v_col0,
-                     long long vectors, int* status) {
+                     unsigned vectors, int* status) {
   constexpr int kLanes = D / 16;
   const int lane = threadIdx.x % kLanes;
-  const long long vec = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  const unsigned vec = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   if (vec >= vectors) return;
-  const int per_row = 2 * c.Hkv;
-  const long long t = vec / per_row;
-  const int which = static_cast<int>(vec - t * per_row);
-  const bool is_v = which >= c.Hkv;
-  const int h = is_v ? which - c.Hkv : which;
-  const int slot = slots[t];
-  if (slot < 0) return;
-  if (slot / c.block_size >= c.num_blocks) {
-    if (lane == 0) report_status(status, kStatusBadIndex);
-    return;
-  }
-  const long long at = (static_cast<long long>(slot / c.block_size) * c.Hkv + h) * c.block_size + slot % c.block_size;
-  uint4* dst = reinterpret_cast<uint4*>(qkv + t * pitch + (is_v ? v_col0 : k_col0) + h * D + lane * 16);
-  const void* src = is_v ? c.v : c.k;
+  const Vector w = vector_at(vec, c.Hkv);
+  const long long at = place_of(c, slots[w.t], w.head, lane == 0, status);
+  if (at < 0) return;
+  uint4* dst = reinterpret_cast<uint4*>(qkv + w.t * pitch + (w.is_v ? v_col0 : k_col0) + w.head * D + lane * 16);
+  const void* src = w.is_v ? c.v : c.k;
   if (k8) {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + at * D + lane * 16);
-    const Kv8Scale s = kv8_scale((is_v ? c.v_scale : c.k_scale)[at]);
-    const uint2 a = kv8_decode4(w.x, s), b = kv8_decode4(w.y, s), d = kv8_decode4(w.z, s), e = kv8_decode4(w.w, s);
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + at * D + lane * 16);
+    const Kv8Scale s = kv8_scale((w.is_v ? c.v_scale : c.k_scale)[at]);
+    const uint2 a = kv8_decode4(x.x, s), b = kv8_decode4(x.y, s), d = kv8_decode4(x.z, s), e = kv8_decode4(x.w, s);
     dst[0] = make_uint4(a.x, a.y, b.x, b.y);
     dst[1] = make_uint4(d.x, d.y, e.x, e.y);
   } else {
@@ -155,14 +169,14 @@ rope_kv8_write_decode_kernel(__nv_bfloat16* __restrict__ qkv, long long pitch, c
 
 }  // namespace
 
+static unsigned blocks_of(unsigned vectors, int lanes) { return (vectors + kThreads / lanes - 1) / (kThreads / lanes); }
+
 void launch_kv8_write(const void* qkv, long long pitch, int k_col0, int v_col0, const int* slots, const PagedCache& c, int T, int* status,
                       cudaStream_t s) {
-  const long long vectors = static_cast<long long>(T) * 2 * c.Hkv;
+  const unsigned vectors = static_cast<unsigned>(T) * 2u * c.Hkv;
   if (vectors == 0) return;
-  const int lanes = c.D / 8;
-  const unsigned blocks = static_cast<unsigned>((vectors * lanes + kThreads - 1) / kThreads);
   const auto run = [&](auto kernel) {
-    kernel<<<blocks, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(qkv), pitch, k_col0, v_col0, slots, c, vectors, status);
+    kernel<<<blocks_of(vectors, c.D / 16), kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(qkv), pitch, k_col0, v_col0, slots, c, vectors, status);
     check_cuda(cudaGetLastError(), "kv8_write");
   };
   if (c.D == 128) run(kv8_write_kernel<128>);
@@ -171,12 +185,10 @@ void launch_kv8_write(const void* qkv, long long pitch, int k_col0, int v_col0, 
 
 void launch_kv_cache_read(const PagedCache& c, const int* slots, void* qkv, long long pitch, int k_col0, int v_col0, int T, int* status,
                           cudaStream_t s) {
-  const long long vectors = static_cast<long long>(T) * 2 * c.Hkv;
+  const unsigned vectors = static_cast<unsigned>(T) * 2u * c.Hkv;
   if (vectors == 0) return;
-  const int lanes = c.D / 16;
-  const unsigned blocks = static_cast<unsigned>((vectors * lanes + kThreads - 1) / kThreads);
   const auto run = [&](auto kernel) {
-    kernel<<<blocks, kThreads, 0, s>>>(c, slots, static_cast<__nv_bfloat16*>(qkv), pitch, k_col0, v_col0, vectors, status);
+    kernel<<<blocks_of(vectors, c.D / 16), kThreads, 0, s>>>(c, slots, static_cast<__nv_bfloat16*>(qkv), pitch, k_col0, v_col0, vectors, status);
     check_cuda(cudaGetLastError(), "kv_cache_read");
   };
   const bool k8 = c.k_scale != nullptr;
