@@ -94,7 +94,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint64_t* p_ready = bars + 14;
   uint64_t* o_done = bars + 16;        // after a piece's last product
   uint64_t* o_free = bars + 18;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* p_half = bars + 20;        // P of the upper 64 keys (bf16 cache)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   int* status = p.a.status;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -108,6 +109,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_ready + i, 4);
+      mbar_init(p_half + i, 4);
       mbar_init(o_done + i, 1);
       mbar_init(o_free + i, 4);
     }
@@ -218,13 +220,13 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       __syncwarp();
     };
-    const auto values = [&](int t, int item, bool first) {  // O_t (+)= P_t V
+    const auto values = [&](int t, int item, int from, bool first) {  // O_t (+)= P_t V, 64 keys from step `from` on
       if (elect_one()) {
         const uint32_t v = aRing + (item % S::kSlots) * S::kSlotBytes;
-#pragma unroll(k8 ? 1 : kBN / 16)
-        for (int i = 0; i < kBN / 16; ++i)
+#pragma unroll(k8 ? 1 : kBN / 32)
+        for (int i = from; i < from + kBN / 32; ++i)
           tc_mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + kColP + i * 8, umma_smem_desc(v + i * 2 * kGroupBytes<D>, 1024, kGroupBytes<D>), kIdescO,
-                        (!first || i > 0) ? 1u : 0u);
+                        (!first || i > from) ? 1u : 0u);
       }
       __syncwarp();
     };
@@ -260,9 +262,17 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         for (int t = 0; t < 2 && ok; ++t) {
           if (j >= end[t]) continue;
           if (j == w.j0 && n_o[t] > 0 && !wait(o_free + t, (n_o[t] - 1) & 1, kStatusWaitTmemEmptyTimeout)) break;
-          if (!wait(p_ready + t, n_p[t]++ & 1, kStatusWaitTmemFullTimeout)) break;
+          // The upper half's products run beside the lower half's exponentials (4096 tokens behind 12288: 694 -> 669 us). 8 bits: no gain, the warps that
+          // convert are behind.
+          if (!wait((k8 ? p_ready : p_half) + t, n_p[t] & 1, kStatusWaitTmemFullTimeout)) break;
           tc_fence_after();
-          values(t, 2 * tile + 1, j == w.j0);
+          values(t, 2 * tile + 1, kBN / 32, j == w.j0);
+          if (!k8) {
+            if (!wait(p_ready + t, n_p[t] & 1, kStatusWaitTmemFullTimeout)) break;
+            tc_fence_after();
+          }
+          ++n_p[t];
+          values(t, 2 * tile + 1, 0, false);
           if (j + 1 >= end[t]) {
             commit(o_done + t);
             ++n_o[t];
@@ -452,6 +462,13 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             }
             tmem_st_32x16(dst, pk);
           };
+          const auto half_done = [&] {
+            if (k8) return;
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_half + t);
+          };
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           if (first_pos < key0 + kBN - 1) {
             // Some row of the warp does not see the whole tile: 32 columns at a time, in a loop. A unit has one or two such tiles; unrolled, their code
@@ -479,6 +496,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
               tc_wait_ld();
               hide(c, s);
               exponentials(s, tS + kColP + c * 16);
+              if (c == 2) half_done();
             }
           } else {
             uint32_t s0[32], s1[32];
@@ -496,6 +514,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             // the upper half first: P lies over it
             exponentials(s0, tS + kColP + 32);
             exponentials(s1, tS + kColP + 48);
+            half_done();
             tmem_ld_32x32(tS, s0);
             tmem_ld_32x32(tS + 32, s1);
             tc_wait_ld();
@@ -503,6 +522,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             exponentials(s1, tS + kColP + 16);
           }
           tc_wait_st();
+        } else if (!k8 && lane == 0) {
+          mbar_arrive(p_half + t);
         }
         tc_fence_before();
         __syncwarp();
