@@ -220,13 +220,16 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       __syncwarp();
     };
-    const auto values = [&](int t, int item, int from, bool first) {  // O_t (+)= P_t V, 64 keys from step `from` on
+    // O_t (+)= P_t V, 16 keys a step. Both caches take a tile's keys from the middle on, then from the beginning: equal values, equal sums.
+    const auto values = [&](auto steps, int t, int item, int from, bool first) {
       if (elect_one()) {
         const uint32_t v = aRing + (item % S::kSlots) * S::kSlotBytes;
-#pragma unroll(k8 ? 1 : kBN / 32)
-        for (int i = from; i < from + kBN / 32; ++i)
+#pragma unroll(k8 ? 1 : decltype(steps)::value)
+        for (int s = 0; s < decltype(steps)::value; ++s) {
+          const int i = (from + s) % (kBN / 16);
           tc_mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + kColP + i * 8, umma_smem_desc(v + i * 2 * kGroupBytes<D>, 1024, kGroupBytes<D>), kIdescO,
-                        (!first || i > from) ? 1u : 0u);
+                        (!first || s > 0) ? 1u : 0u);
+        }
       }
       __syncwarp();
     };
@@ -264,15 +267,16 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           if (j == w.j0 && n_o[t] > 0 && !wait(o_free + t, (n_o[t] - 1) & 1, kStatusWaitTmemEmptyTimeout)) break;
           // The upper half's products run beside the lower half's exponentials (4096 tokens behind 12288: 694 -> 669 us). 8 bits: no gain, the warps that
           // convert are behind.
-          if (!wait((k8 ? p_ready : p_half) + t, n_p[t] & 1, kStatusWaitTmemFullTimeout)) break;
-          tc_fence_after();
-          values(t, 2 * tile + 1, kBN / 32, j == w.j0);
+          using Half = std::integral_constant<int, kBN / 32>;
           if (!k8) {
-            if (!wait(p_ready + t, n_p[t] & 1, kStatusWaitTmemFullTimeout)) break;
+            if (!wait(p_half + t, n_p[t] & 1, kStatusWaitTmemFullTimeout)) break;
             tc_fence_after();
+            values(Half{}, t, 2 * tile + 1, kBN / 32, j == w.j0);
           }
-          ++n_p[t];
-          values(t, 2 * tile + 1, 0, false);
+          if (!wait(p_ready + t, n_p[t]++ & 1, kStatusWaitTmemFullTimeout)) break;
+          tc_fence_after();
+          if (k8) values(std::integral_constant<int, kBN / 16>{}, t, 2 * tile + 1, kBN / 32, j == w.j0);
+          else values(Half{}, t, 2 * tile + 1, 0, false);
           if (j + 1 >= end[t]) {
             commit(o_done + t);
             ++n_o[t];
