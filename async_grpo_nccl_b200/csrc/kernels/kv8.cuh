@@ -52,6 +52,16 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
+// a * 0 + b, for both halves: a NaN where a is infinite or none, for b = 0 and for b that came of this.
+__device__ __forceinline__ uint32_t times_zero(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(b));
+  return d;
+}
+
+__device__ __forceinline__ bool is_finite(uint32_t half) { return (half & 0x7f80u) != 0x7f80u; }  // of a bf16 value in the lower half
+__device__ __forceinline__ uint32_t only_finite(uint32_t x) { return (is_finite(x) ? x & 0xffffu : 0u) | (is_finite(x >> 16) ? x & 0xffff0000u : 0u); }
+
 // Factors (both halves of a word) that turn codes moved into bf16's exponent field into what they stand for. An e4m3 code moved there is
 // 2^-120 of its value, subnormals included (bias 127 against 7); 2^120 * 2^e is a bf16 number up to e = 7, beyond that a second
 // factor follows.

@@ -43,7 +43,8 @@ struct Shape {
   static constexpr int kRaw = k8 ? 2 : 0;                     // tiles of codes under way: one of K, one of V
   static constexpr int kMmaWarp = 8, kLoadWarp = 9;
   static constexpr int kConvWarp = 12;                        // 8 bits: five warpgroups, registers dealt out anew; warps 10 and 11 do nothing
-  static constexpr int kThreads = k8 ? 640 : 320;
+  static constexpr int kCleanWarp = 10;                       // bf16
+  static constexpr int kThreads = k8 ? 640 : 352;
   static constexpr int kRingOff = kQBytes;
   static constexpr int kRawOff = kRingOff + kSlots * kSlotBytes;
   static constexpr int kScaleOff = kRawOff + kRaw * kBN * D;
@@ -72,6 +73,89 @@ __device__ __forceinline__ void take_registers() {
   if (kOn) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMore));
 }
 
+// Pieces from, from + 32, .. of a bf16 tile of V: piece i is row i / 8, bytes (i % 8) * 16 of its atoms.
+template <int D>
+__device__ __forceinline__ uint4* piece(uint8_t* v, int i) {
+  return reinterpret_cast<uint4*>(v + (i >> 6) * kGroupBytes<D> + (i & 63) * 16);
+}
+template <int D>
+__device__ __forceinline__ bool some_odd(uint8_t* v, int from, int end) {
+  uint32_t nan = 0u;
+#pragma unroll 1
+  for (int i = from; i < end; i += 32) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      const uint4 y = piece<D>(v, i)[c * 64];
+      nan = times_zero(y.x, times_zero(y.y, times_zero(y.z, times_zero(y.w, nan))));
+    }
+  }
+  return (nan & 0x7fff7fffu) != 0u;
+}
+template <int D>
+__device__ __noinline__ void only_finite_rows(uint8_t* v, int from, int end) {
+  for (int i = from; i < end; i += 32) {
+    for (int c = 0; c < D / 64; ++c) {
+      const uint4 y = piece<D>(v, i)[c * 64];
+      piece<D>(v, i)[c * 64] = make_uint4(only_finite(y.x), only_finite(y.y), only_finite(y.z), only_finite(y.w));
+    }
+  }
+}
+// What was taken out of the products, at a piece's end: values that are no numbers at the keys from .. to - 1, for the rows that see them (up to `pos`). Adds them
+// to O (a warp's rows, `tO` in tensor memory); 8 bits, where a vector that holds a NaN is all NaN: returns one in place of the row's sum l. Apart from the kernel's
+// code, whose size counts.
+template <int D, bool k8>
+__device__ __noinline__ float add_taken_out(const LineParams& p, int b, int kvh, int from, int to, int pos, uint32_t tO, float l) {
+  const auto row_of = [&](int key) -> long long {
+    const int page = p.a.block_tables[b * p.a.table_pitch + key / p.c.block_size];
+    if (page < 0 || page >= p.c.num_blocks) return -1;
+    return (static_cast<long long>(page) * p.c.Hkv + kvh) * p.c.block_size + (key & (p.c.block_size - 1));
+  };
+  if (k8) {
+    for (int key = from; key < min(to, pos + 1); ++key) {
+      const long long row = row_of(key);
+      if (row >= 0 && p.c.v_scale[row] == kKv8NanByte) l = __uint_as_float(0x7fffffffu);
+    }
+    __syncwarp();
+    return l;
+  }
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld_32x32(tO + c * 32, o);
+    tc_wait_ld();
+#pragma unroll 1
+    for (int key = from; key < to; ++key) {
+      const long long row = row_of(key);
+      if (row < 0 || key > pos) continue;
+      const auto* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.c.v) + row * D + c * 32);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 x = src[i];
+        const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float lo = __uint_as_float(o[i * 8 + 2 * k]), hi = __uint_as_float(o[i * 8 + 2 * k + 1]);
+          if (!is_finite(y[k])) lo += __uint_as_float(y[k] << 16);
+          if (!is_finite(y[k] >> 16)) hi += __uint_as_float(y[k] & 0xffff0000u);
+          o[i * 8 + 2 * k] = __float_as_uint(lo);
+          o[i * 8 + 2 * k + 1] = __float_as_uint(hi);
+        }
+      }
+    }
+    __syncwarp();
+    uint32_t lo[16], hi[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      lo[i] = o[i];
+      hi[i] = o[16 + i];
+    }
+    tmem_st_32x16(tO + c * 32, lo);
+    tmem_st_32x16(tO + c * 32 + 16, hi);
+  }
+  tc_wait_st();
+  return l;
+}
+
 template <int D, bool k8>
 __global__ void __launch_bounds__(Shape<D, k8>::kThreads, 1)
 paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -95,14 +179,17 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint64_t* o_done = bars + 16;        // after a piece's last product
   uint64_t* o_free = bars + 18;
   uint64_t* p_half = bars + 20;        // P of the upper 64 keys (bf16 cache)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  uint64_t* cleaned = bars + 22;       // [kSlots], bf16: V of a tile that had to be cleaned is
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
+  volatile int* odd = reinterpret_cast<volatile int*>(bars + 28);  // set once a value was taken out of the products
   int* status = p.a.status;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(full + i, k8 ? 4 : 1);
-      mbar_init(empty + i, 1);
+      mbar_init(empty + i, k8 ? 1 : 2);
+      mbar_init(cleaned + i, 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -114,6 +201,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       mbar_init(o_free + i, 4);
     }
     fence_mbar_init();
+    *odd = 0;
   }
   if (warp == S::kMmaWarp) {
     tmem_alloc(tmem_slot, 512);
@@ -132,6 +220,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const uint32_t tmem = *tmem_slot;
   Walk<kBN, kExtra> w;  // every warp walks by itself
   w.start(p, share, near);
+  const auto to_clean = [](int j, int keys, int hidden) { return keys < (j + 1) * kBN || hidden < (j + 1) * kBN; };
 
   if (warp == S::kLoadWarp) {
     give_registers<k8, 64>();
@@ -198,6 +287,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     int tile = 0, n_q = 0;          // tiles and pieces so far
     int n_p[2] = {0, 0};            // of each tile of Q: softmaxes waited for
     int n_o[2] = {0, 0};            // pieces finished
+    uint32_t n_clean = 0;           // of each slot: parity of its cleanings (a bit)
     bool ok = true;
     const auto wait = [&](uint64_t* bar, int parity, int code) {
       if (ok && !mbar_wait(bar, parity)) {
@@ -237,19 +327,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       if (elect_one()) tc_commit(bar);
       __syncwarp();
     };
-    // Rows of V behind the last visible key: whatever the page held before, 0 * NaN would reach every row. (The converting warps do it for 8 bits.)
-    const auto clear_tail = [&](int item, int valid) {
-      if (k8 || valid >= kBN) return;
-      uint8_t* v = ring + (item % S::kSlots) * S::kSlotBytes;
-      for (int i = max(valid, 0) * 8 + lane; i < kBN * 8; i += 32) {  // row i / 8, bytes (i % 8) * 16 of its atoms
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(v + (i >> 6) * kGroupBytes<D> + c * 1024 + (i & 63) * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
     for (; w.more() && ok; w.next(p)) {
-      const int keys = unit_keys(p, w.s, w.qb);
+      const int keys = unit_keys(p, w.s, w.qb), hidden = first_hidden(p, w.s, w.qb);
       if (!wait(q_full, n_q++ & 1, kStatusWaitFullTimeout)) break;
       const int end[2] = {w.end_of(p, 0), w.end_of(p, 1)};
       if (!slot_wait(2 * tile)) break;
@@ -261,7 +340,14 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const bool more = j + 1 < w.j1;
         if (!more) commit(q_empty);
         if (!slot_wait(2 * tile + 1)) break;
-        clear_tail(2 * tile + 1, keys - j * kBN);
+        bool cleaning = !k8 && to_clean(j, keys, hidden);
+        const auto is_clean = [&] {
+          const int slot = (2 * tile + 1) % S::kSlots;
+          if (cleaning) wait(cleaned + slot, (n_clean >> slot) & 1, kStatusWaitFullTimeout);
+          if (cleaning) n_clean ^= 1u << slot;
+          cleaning = false;
+          return ok;
+        };
         for (int t = 0; t < 2 && ok; ++t) {
           if (j >= end[t]) continue;
           if (j == w.j0 && n_o[t] > 0 && !wait(o_free + t, (n_o[t] - 1) & 1, kStatusWaitTmemEmptyTimeout)) break;
@@ -269,7 +355,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           // convert are behind.
           using Half = std::integral_constant<int, kBN / 32>;
           if (!k8) {
-            if (!wait(p_half + t, n_p[t] & 1, kStatusWaitTmemFullTimeout)) break;
+            if (!wait(p_half + t, n_p[t] & 1, kStatusWaitTmemFullTimeout) || !is_clean()) break;
             tc_fence_after();
             values(Half{}, t, 2 * tile + 1, kBN / 32, j == w.j0);
           }
@@ -286,10 +372,51 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             scores(t, 2 * tile + 2);
           }
         }
+        if (!is_clean()) break;
         commit(empty + (2 * tile + 1) % S::kSlots);
         if (more) {
           slot_wait(2 * tile + 2);  // where no tile of Q takes part any more, it still counts as read
           commit(empty + (2 * tile + 2) % S::kSlots);
+        }
+      }
+    }
+  } else if (!k8 && warp >= S::kCleanWarp) {
+    // ---------------------------------------------------------------- values that must not meet a probability of zero
+    // Rows of V behind the last key (whatever the page held before) become zero, and so do values that are no numbers at keys that some rows do not see. A
+    // warp for that, as soon as V is there: the warp that issues the products took 8 us of 85 for it (9 prompts of 16 to 1500 tokens), this one 3. It takes part
+    // in the release of every slot, so that it is never a round of the ring ahead or behind.
+    int item = 0;
+    bool ok = true;
+    for (; w.more() && ok; w.next(p)) {
+      const int keys = unit_keys(p, w.s, w.qb), hidden = first_hidden(p, w.s, w.qb);
+      for (int i = 2 * w.j0; i < 2 * w.j1; ++i, ++item) {
+        const int slot = item % S::kSlots, j = i >> 1;
+        if (!mbar_wait(full + slot, (item / S::kSlots) & 1)) {
+          report_status(status, kStatusWaitFullTimeout);
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        if (!(i & 1) || !to_clean(j, keys, hidden)) {
+          if (lane == 0) mbar_arrive(empty + slot);
+          continue;
+        }
+        uint8_t* v = ring + slot * S::kSlotBytes;
+        const int from = max(hidden - j * kBN, 0), end = max(min(keys - j * kBN, kBN), 0);
+        if (some_odd<D>(v, from * 8 + lane, end * 8)) {
+          only_finite_rows<D>(v, from * 8 + lane, end * 8);
+          *odd = 1;
+        }
+#pragma unroll 1
+        for (int i = end * 8 + lane; i < kBN * 8; i += 32) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) piece<D>(v, i)[c * 64] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(cleaned + slot);
+          mbar_arrive(empty + slot);
         }
       }
     }
@@ -356,7 +483,13 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         __syncwarp();
         // of row 32 (lane / 8) + 8 cw + lane % 8. Behind the last key the codes are zero, and the factor has to be a number
         const int left = unit_keys(p, w.s, w.qb) - j * kBN - cw * 8;
-        const Kv8Scale s = kv8_scale((lane >> 3) * 32 + (lane & 7) < left ? raw_scale[lane] : 0);
+        const int r = (lane >> 3) * 32 + (lane & 7);
+        int byte = r < left ? raw_scale[lane] : 0;
+        if (v && byte == kKv8NanByte && j * kBN + cw * 8 + r >= first_hidden(p, w.s, w.qb)) {
+          byte = 0;
+          *odd = 1;
+        }
+        const Kv8Scale s = kv8_scale(byte);
         const bool twice = __any_sync(0xffffffffu, s.twice);         // some value above 448 * 2^7
         if (round > 0 && !mbar_wait(empty + slot, (round - 1) & 1)) {
           report_status(status, kStatusWaitEmptyTimeout);
@@ -534,7 +667,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         if (lane == 0) mbar_arrive(p_ready + t);
       }
       if (!ok) break;
-      const float l = l2.x + l2.y;
+      float l = l2.x + l2.y;
       const bool any = end > w.j0;  // else O holds nothing of this piece
       if (any && !mbar_wait(o_done + t, n_o++ & 1)) {
         report_status(status, kStatusWaitTmemFullTimeout);
@@ -542,6 +675,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         break;
       }
       tc_fence_after();
+      if (any && busy && *odd != 0)
+        l = add_taken_out<D, k8>(p, w.b, w.kvh, max(first_hidden(p, w.s, w.qb), w.j0 * kBN), min(unit_keys(p, w.s, w.qb), w.j1 * kBN), pos, tO, l);
       if (busy) {
         const bool whole = w.whole(), valid = r < rows;
         // a lane's stores are a row of their own: whole 32-byte sectors where the output's rows allow it

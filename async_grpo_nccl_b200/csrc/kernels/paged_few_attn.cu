@@ -245,6 +245,8 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
+    const int hidden = first_hidden(p, w.s, w.qb);
+    bool odd = false;              // a value was taken out of the products
     int v_pow = 0, v_first = 0;    // 8 bits: F + 127, at first; O is held in 2^F
 
     for (int j = w.j0; j < w.j1; ++j) {
@@ -348,6 +350,17 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
           return !__any_sync(0xffffffffu, (((f[0] + c) | (f[1] + c)) & 0xfff0fff0u) != 0u);
         };
         bool good = fits();
+        if (!good && hidden < keys && (j + 1) * kKeys > hidden) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int shift = 16 * (h & 1);
+            if (((f[h >> 1] >> shift) & 0xffffu) != kKv8NanByte || j * kKeys + 2 * t + (h & 1) + 8 * (h >> 1) < hidden) continue;
+            f[h >> 1] &= 0xffff0000u >> shift;
+            odd = true;
+#pragma unroll
+            for (int i = 0; i < kVW; ++i) v[h][i] = 0u;
+          }
+        }
         if (!good) {  // another F: the largest byte, without those of NaN
           const auto real = [](uint32_t x) { return x == 255u ? 0u : x; };
           const uint32_t mine = max(max(real(f[0] & 0xffffu), real(f[0] >> 16)), max(real(f[1] & 0xffffu), real(f[1] >> 16)));
@@ -415,6 +428,18 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
           }
         }
       } else {
+        if (hidden < keys && (j + 1) * kKeys > hidden) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t nan = 0u;
+#pragma unroll
+            for (int i = 0; i < kVW; ++i) nan = times_zero(v[h][i], nan);
+            if ((nan & 0x7fff7fffu) == 0u || j * kKeys + 2 * t + (h & 1) + 8 * (h >> 1) < hidden) continue;
+            odd = true;
+#pragma unroll
+            for (int i = 0; i < kVW; ++i) v[h][i] = only_finite(v[h][i]);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
           uint32_t a[4];
@@ -434,6 +459,29 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
     }
 
     // ---- the piece's end
+    if (__any_sync(0xffffffffu, odd)) {
+      const int last = min(keys, w.j1 * kKeys);
+#pragma unroll 1
+      for (int key = max(hidden, w.j0 * kKeys); key < last; ++key) {
+        const int page = table[key / bs];
+        if (page < 0 || page >= p.c.num_blocks) continue;
+        const long long row = (static_cast<long long>(page) * Hkv + w.kvh) * bs + (key & (bs - 1));
+        const bool nan = k8 && p.c.v_scale[row] == kKv8NanByte;
+        const auto* src = reinterpret_cast<const uint32_t*>(v_lane - 2 * t * kRow + row * kRow);
+        const int rows_from = (key - first_pos) * G;  // the rows that see it
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const uint32_t x = k8 ? (nan ? 0x7fff7fffu : 0u) : src[i % 4 + i / 4 * 32];
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              const uint32_t half = d < 2 ? x << 16 : x & 0xffff0000u;
+              if (!is_finite(half >> 16) && 8 * n + 2 * t + (d & 1) >= rows_from) o[n][i][d] += __uint_as_float(half);
+            }
+        }
+      }
+    }
     const bool whole = w.whole();
     const int part = w.part(warp) * F::kRows;
     const float unit = k8 ? power(v_pow) : 1.f;

@@ -69,6 +69,9 @@ struct SeqCache {
 };
 // Keys that the last row of unit qb sees, and tiles of them. A unit without keys still has a tile: its rows are zeros to be written.
 __device__ __forceinline__ int unit_keys(const LineParams& p, const Seq& s, int qb) { return max(s.len - s.n + min(s.n, (qb + 1) * p.tokens), 0); }
+// Keys from here on are hidden from some of a unit's rows. A value there that is infinite or no number would reach those rows by 0 * NaN: the kernels take it
+// out of the products, and add it at the end to the rows that see it.
+__device__ __forceinline__ int first_hidden(const LineParams& p, const Seq& s, int qb) { return max(s.len - s.n + qb * p.tokens + 1, 0); }
 template <int kKeys>
 __device__ __forceinline__ int unit_tiles(const LineParams& p, const Seq& s, int qb) {
   return max(1, (unit_keys(p, s, qb) + kKeys - 1) / kKeys);

@@ -168,6 +168,44 @@ def test_a_nan_stays_with_the_rows_that_see_it(seqs, eight):
 
 
 @pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D", [(12, 2, 128), (8, 1, 64), (3, 3, 128), (20, 2, 64)])
+@pytest.mark.parametrize("seqs", [[(3, 40), (2, 700), (5, 5)], [(1, 300), (2, 3), (1, 17)], [(60, 300), (200, 500), (9, 3)], [(300, 2300), (300, 300)]])
+def test_values_that_are_no_numbers_do_not_reach_rows_that_do_not_see_them(seqs, Hq, Hkv, D, eight):
+    """NaN and infinite values at tokens that some rows see and others do not: those rows are as if the values were zero, the others not finite
+    in the places that the values have."""
+    c = Case(seqs, Hq, Hkv, D, 16, eight, seed=13)
+    clean = c.values[1].clone()
+    bad = torch.zeros(clean.shape, dtype=torch.bool, device=DEV)
+    for b, (n, total) in enumerate(seqs):
+        for back, kind in ((1, math.inf), (1 + n // 2, math.nan), (max(n - 1, 1), -math.inf)):
+            token = total - back
+            if not 0 <= token or back >= n:
+                continue
+            page, off, h = int(c.table[b, token // 16]), token % 16, b % Hkv
+            if eight:
+                c.scales[1][page, h, off] = 255
+                c.kv[1].view(torch.uint8)[page, h, off] = 0
+                bad[page, h, off] = True
+                clean[page, h, off] = 0
+            else:
+                for d in (back % D, D - 1):
+                    c.kv[1][page, h, off, d] = kind
+                    bad[page, h, off, d] = True
+                    clean[page, h, off, d] = 0
+    assert bool(bad.any())
+    c.call()
+    want, size = R.paged_chunk_attention(c.rows, c.values[0], clean, c.table, c.lens, c.starts, Hq, Hkv, D, 1 / math.sqrt(D))
+    # the largest probability-weighted sum of marks: what sees one has a number above zero there
+    marks, _ = R.paged_chunk_attention(c.rows, torch.zeros_like(c.values[0]), bad.double(), c.table, c.lens, c.starts, Hq, Hkv, D, 1.0)
+    seen = marks > 0
+    assert bool(seen.any()) and bool((~seen).any())
+    assert bool((c.out.isfinite() == ~seen).all())
+    off = (c.out.double() - want).abs() - (want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -10))
+    assert float(off[~seen].max()) <= 0
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("eight", [False, True])
 def test_queries_of_any_size(eight):
     """Rows of Q from subnormal to 2^60, one of zeros: with keys as small as the queries are large, logits stay moderate."""
     for n in (1, 50):
