@@ -101,6 +101,38 @@ kv_cache_read_kernel(PagedCache c, const int* __restrict__ slots, __nv_bfloat16*
   }
 }
 
+// One CTA: 16 tokens of a sequence, all heads of K and V.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv8_unpack_kernel(const __grid_constant__ ChunkAttnArgs a, PagedCache c, PagedCache to, int* __restrict__ table) {
+  constexpr int kLanes = D / 16;
+  pdl_wait();
+  pdl_launch();
+  const int per_page = c.block_size / 16;
+  const int at = blockIdx.x / per_page, part = blockIdx.x - at * per_page;  // block of the new cache
+  const int b = at / a.max_blocks, i = at - b * a.max_blocks;
+  if (i * c.block_size + part * 16 >= a.seq_lens[b] || a.q_starts[b + 1] == a.q_starts[b]) return;
+  int page = a.block_tables[b * a.table_pitch + i];
+  if (page < 0 || page >= c.num_blocks) {
+    if (threadIdx.x == 0) report_status(a.status, kStatusBadIndex);
+    page = 0;
+  }
+  if (threadIdx.x == 0 && part == 0) table[at] = at;
+  const int lane = threadIdx.x % kLanes;
+#pragma unroll 4
+  for (int vec = threadIdx.x / kLanes; vec < 2 * c.Hkv * 16; vec += kThreads / kLanes) {  // 16 tokens of a head of K, .. of V
+    const bool is_v = vec >= c.Hkv * 16;
+    const int head = (vec >> 4) - (is_v ? c.Hkv : 0);
+    const long long in_page = static_cast<long long>(head) * c.block_size + part * 16 + (vec & 15);
+    const long long src = static_cast<long long>(page) * c.Hkv * c.block_size + in_page, dst = static_cast<long long>(at) * c.Hkv * c.block_size + in_page;
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(is_v ? c.v : c.k) + src * D + lane * 16);
+    const Kv8Scale s = kv8_scale((is_v ? c.v_scale : c.k_scale)[src]);
+    const uint2 d = kv8_decode4(x.x, s), e = kv8_decode4(x.y, s), f = kv8_decode4(x.z, s), g = kv8_decode4(x.w, s);
+    uint4* y = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(is_v ? to.v : to.k) + dst * D + lane * 16);
+    y[0] = make_uint4(d.x, d.y, e.x, e.y);
+    y[1] = make_uint4(f.x, f.y, g.x, g.y);
+  }
+}
+
 // One CTA a row; D / 16 lanes a head, each with 8 values of the lower half of the head and the 8 that they are rotated with. The rotated
 // key is rounded to bf16, as the row keeps it, before it is quantised: a token's entry is the same from a decode step as from a prefill.
 template <int D>
@@ -211,6 +243,12 @@ void launch_rope_kv8_write_decode(void* qkv, long long pitch, const float* cos_t
     AGRPO_PREFER_SMEM(rope_kv8_write_decode_kernel<64>);
     run(rope_kv8_write_decode_kernel<64>);
   }
+}
+
+void launch_kv8_unpack(const ChunkAttnArgs& a, const PagedCache& c, const PagedCache& to, int* table, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(to.num_blocks * (c.block_size / 16)));
+  if (c.D == 128) launch_kernel(kv8_unpack_kernel<128>, grid, dim3(kThreads), 0, s, "kv8_unpack", a, c, to, table);
+  else launch_kernel(kv8_unpack_kernel<64>, grid, dim3(kThreads), 0, s, "kv8_unpack", a, c, to, table);
 }
 
 }  // namespace agrpo

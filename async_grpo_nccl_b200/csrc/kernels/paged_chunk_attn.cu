@@ -7,8 +7,8 @@
 // the two products of a tile).
 //
 // A unit is two tiles of 128 rows, which share the keys and values. S = Q K^T and O += P V run on tcgen05 with S, P and O in tensor memory, a thread a row; one
-// tile's softmax runs beside the other's products. Keys and values come page by page into a ring. 8-bit cache: four warps bring the codes into shared memory, each
-// thread what it will need, and turn them into the bf16 tiles that the products read (kv8.cuh).
+// tile's softmax runs beside the other's products. Keys and values come page by page into a ring. 8-bit cache: eight warps bring the codes into shared memory, each
+// thread what it will need, and turn them into the bf16 tiles that the products read (kv8.cuh); for sequences of many rows that is done once, ahead (kUnpackRows).
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -383,7 +383,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   } else if (!k8 && warp >= S::kCleanWarp) {
     // ---------------------------------------------------------------- values that must not meet a probability of zero
     // Rows of V behind the last key (whatever the page held before) become zero, and so do values that are no numbers at keys that some rows do not see. A
-    // warp for that, as soon as V is there: the warp that issues the products took 8 us of 85 for it (9 prompts of 16 to 1500 tokens), this one 3. It takes part
+    // warp for that, as soon as V is there: the warp that issues the products took 8 us of 85 for it (24 sequences of up to 900 new tokens), this one 3. It takes part
     // in the release of every slot, so that it is never a round of the ring ahead or behind.
     int item = 0;
     bool ok = true;
@@ -771,10 +771,31 @@ int unit_rows(const ChunkAttnArgs& a, const PagedCache& c) {
   return G <= 16 && rows <= 16ll * a.B ? 16 : 256;
 }
 
+// An 8-bit cache is converted to bf16 once, ahead of the attention, where every key would otherwise be converted for four units or more (on average): a tile of keys
+// takes a unit 1.4 times as long from 8 bits as from bf16, and writing it out as long as a third of such a tile. 4096 rows of 28 heads behind 12288 tokens
+// 955 -> 676 us; four units over 16000 tokens 51.4 -> 49.8, three 51.5 -> 54. Up to about the size of L2, where the copy stays; it is the allocator's again
+// after the call.
+constexpr long long kUnpackMost = 128ll << 20;
+constexpr long long kUnpackRows = 1024;  // of a sequence
+struct Unpacked {
+  long long table = 0, cache = 0;  // bytes; 0: the keys are converted by the attention
+};
+Unpacked unpacked(const ChunkAttnArgs& a, const PagedCache& c) {
+  Unpacked u;
+  const long long blocks = static_cast<long long>(a.B) * a.max_blocks;
+  const long long bytes = blocks * c.Hkv * c.block_size * c.D * 2;
+  if (c.k_scale == nullptr || static_cast<long long>(a.Tq) * (a.Hq / c.Hkv) < kUnpackRows * a.B || 2 * bytes > kUnpackMost) return u;
+  u.table = (blocks * 4 + 255) / 256 * 256;
+  u.cache = bytes;
+  return u;
+}
+
 }  // namespace
 
 long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, int num_sms) {
-  return line_scratch(num_sms, unit_rows(a, c), c.D);
+  const long long line = line_scratch(num_sms, unit_rows(a, c), c.D);
+  const Unpacked u = unpacked(a, c);
+  return u.cache ? (line + 255) / 256 * 256 + u.table + 2 * u.cache : line;
 }
 
 void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int num_sms, void* scratch, cudaStream_t s) {
@@ -786,6 +807,18 @@ void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int nu
   p.c = c;
   p.G = a.Hq / c.Hkv;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const Unpacked u = unpacked(a, c);
+  if (u.cache) {
+    auto* table = static_cast<uint8_t*>(scratch) + (line_scratch(num_sms, rows, c.D) + 255) / 256 * 256;
+    p.c.k = table + u.table;
+    p.c.v = table + u.table + u.cache;
+    p.c.k_scale = p.c.v_scale = nullptr;
+    p.c.num_blocks = a.B * a.max_blocks;
+    p.a.block_tables = reinterpret_cast<int*>(table);
+    p.a.table_pitch = a.max_blocks;
+    launch_kv8_unpack(a, c, p.c, reinterpret_cast<int*>(table), s);
+    return c.D == 128 ? launch<128, false>(p, num_sms, scratch, s) : launch<64, false>(p, num_sms, scratch, s);
+  }
   const bool k8 = c.k_scale != nullptr;
   if (c.D == 128) k8 ? launch<128, true>(p, num_sms, scratch, s) : launch<128, false>(p, num_sms, scratch, s);
   else k8 ? launch<64, true>(p, num_sms, scratch, s) : launch<64, false>(p, num_sms, scratch, s);

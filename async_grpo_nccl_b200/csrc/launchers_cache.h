@@ -43,6 +43,10 @@ struct ChunkAttnArgs {
 long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, int num_sms);
 void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int num_sms, void* scratch, cudaStream_t s);
 
+// An 8-bit cache in bf16, for the sequences that have rows: block i of sequence b is block b * max_blocks + i of `to` (with its num_blocks set by the caller), which
+// is what `table` [B, max_blocks] says afterwards. Blocks behind a sequence's tokens are left as they are.
+void launch_kv8_unpack(const ChunkAttnArgs& a, const PagedCache& c, const PagedCache& to, int* table, cudaStream_t s);
+
 // Its form for units of up to 8 or 16 rows (paged_few_attn.cu).
 void launch_paged_few_attn(const ChunkAttnArgs& a, const PagedCache& c, int rows, int num_sms, void* scratch, cudaStream_t s);
 

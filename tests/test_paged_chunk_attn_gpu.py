@@ -149,7 +149,7 @@ def test_values_that_grow_along_the_sequence(seqs):
 
 
 @pytest.mark.parametrize("eight", [False, True])
-@pytest.mark.parametrize("seqs", [[(1, 300), (1, 300)], [(70, 300), (70, 300)]])
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 300)], [(70, 300), (70, 300)], [(200, 300), (200, 300)]])
 def test_a_nan_stays_with_the_rows_that_see_it(seqs, eight):
     """A key or a value that is NaN makes its own sequence's rows NaN, those that see it and no other sequence's."""
     for i in range(2):
@@ -276,6 +276,71 @@ def test_captured_calls_follow_the_lengths(eight):
     torch.cuda.synchronize()
     for c in cases + [eager]:
         c.check()
+
+
+def test_captured_calls_with_a_converted_copy():
+    """Two graphs of many rows over 8 bits replayed on two streams at once, and an eager call on a third, lengths changed in between."""
+    cases = [Case([(n, 1500), (900, 1000)], 12, 2, 128, 16, True, seed=n) for n in (600, 800, 1000)]
+    graphs = []
+    for c in cases[:2]:
+        c.call()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.call()
+        graphs.append(g)
+    cases[0].lens.copy_(torch.tensor([700, 901]))
+    cases[1].lens.copy_(torch.tensor([30, 0]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(4):
+        for s, f in zip(streams, (graphs[0].replay, graphs[1].replay, cases[2].call)):
+            with torch.cuda.stream(s):
+                f()
+    torch.cuda.synchronize()
+    for c in cases:
+        c.check()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,bs", [(12, 2, 128, 16), (6, 3, 64, 64), (8, 8, 128, 128)])
+def test_the_converted_copy_of_an_eight_bit_cache(Hq, Hkv, D, bs):
+    """Many rows a sequence: the cache is converted once, ahead. With a table so wide that the copy would be too large the attention converts the keys itself; both
+    give the same bits."""
+    seqs = [(1100, 1200), (0, 500), (1, 300), (2200, 2200), (40, 0), (0, 0)]
+    c = Case(seqs, Hq, Hkv, D, bs, True, pad=3, pitch=64, seed=21)
+    c.call()
+    c.check()
+    first = c.out.clone()
+    wide = torch.full((len(seqs), (128 << 20) // (len(seqs) * 4 * Hkv * bs * D) + 1), 2 ** 30, dtype=torch.int32, device=DEV)
+    wide[:, :c.table.shape[1]] = c.table
+    c.table = wide
+    c.out.fill_(7)
+    c.call()
+    c.check()
+    assert torch.equal(c.out, first)
+
+
+def test_a_page_that_does_not_exist_under_many_rows():
+    c = Case([(700, 700), (900, 1000)], 12, 2, 128, 16, True)
+    c.call()
+    first = c.out.clone()
+    page = int(c.table[0, 7])
+    for bad in (-1, 10 ** 6):
+        c.table[0, 7] = bad
+        c.out.fill_(7)
+        c.call()
+        assert int(c.status) == 6
+        c.status.zero_()
+        assert torch.equal(c.out[700:], first[700:]) and torch.equal(c.out[:7 * 16], first[:7 * 16])
+    c.table[0, 7] = page
+    c.lens[0] = 2 ** 30  # more than its table holds
+    c.call()
+    assert int(c.status) == 6
+    c.status.zero_()
+    c.lens[0] = 700
+    c.out.fill_(7)
+    c.call()
+    assert int(c.status) == 0 and torch.equal(c.out, first)
 
 
 def test_pages_and_lengths_that_do_not_exist_are_reported():
