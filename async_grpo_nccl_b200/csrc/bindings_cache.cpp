@@ -69,6 +69,7 @@ void paged_chunk_attn(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_
   a.softmax_scale = (float)softmax_scale;
   a.status = int_ptr(status);
   if (a.Tq == 0 || a.B == 0) return;
+  TORCH_CHECK(agrpo::paged_chunk_attn_tiles(a, c) < (int64_t(1) << 31), op, ": too many rows for tables of this width");
   if (a.Tq == 1) a.ldq = Hq * D;  // the pitch of a single row means nothing
   // Parts of units that several CTAs share: from the allocator, so that calls on several streams or in several graphs do not meet in it.
   const int sms = launch_num_sms();

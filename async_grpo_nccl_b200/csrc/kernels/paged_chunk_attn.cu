@@ -11,6 +11,7 @@
 // thread what it will need, and turn them into the bf16 tiles that the products read (kv8.cuh); for sequences of many rows that is done once, ahead (kUnpackRows).
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "../common/f32x2.cuh"
@@ -791,6 +792,13 @@ Unpacked unpacked(const ChunkAttnArgs& a, const PagedCache& c) {
 }
 
 }  // namespace
+
+long long paged_chunk_attn_tiles(const ChunkAttnArgs& a, const PagedCache& c) {
+  const int rows = unit_rows(a, c), G = a.Hq / c.Hkv;
+  const long long units = a.Tq / (rows == 256 ? 2 * (128 / G) : rows / G) + std::min(a.B, a.Tq);
+  const long long keys = static_cast<long long>(a.max_blocks) * c.block_size;
+  return units * c.Hkv * (rows == 256 ? keys / kBN + 2 : keys / 16 + 6);  // with each one's beginning, and a tile that is not full
+}
 
 long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, int num_sms) {
   const long long line = line_scratch(num_sms, unit_rows(a, c), c.D);

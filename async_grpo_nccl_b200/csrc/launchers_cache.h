@@ -39,6 +39,8 @@ struct ChunkAttnArgs {
   float softmax_scale;
   int* status;
 };
+// Tiles of keys that the call has at most, if every table is full: has to be below 2^31.
+long long paged_chunk_attn_tiles(const ChunkAttnArgs& a, const PagedCache& c);
 // `scratch` holds paged_chunk_attn_scratch bytes, 16-byte aligned, and belongs to the call.
 long long paged_chunk_attn_scratch(const ChunkAttnArgs& a, const PagedCache& c, int num_sms);
 void launch_paged_chunk_attn(const ChunkAttnArgs& a, const PagedCache& c, int num_sms, void* scratch, cudaStream_t s);

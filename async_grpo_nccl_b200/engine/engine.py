@@ -436,7 +436,7 @@ class RolloutEngine:
             upto = ends - first[g0:g1] + np.asarray(cached[g0:g1])               # tokens that the prompts have in the cache after it
             done = [int(e) - a - 1 for e, f in zip(ends, first[g0 + 1:g1 + 1]) if e == f]
             words += [starts.astype(np.int32), upto.astype(np.int32), np.asarray(done, dtype=np.int32)]
-            portions.append((a, z, g0, g1, at, len(done)))
+            portions.append((a, z, g0, g1, at, len(done), -(-int(upto.max()) // self.block_size)))
             at += len(starts) + len(upto) + len(done)
         host = torch.from_numpy(np.concatenate(words)).pin_memory()
         d = host.to(self.dev, non_blocking=True)
@@ -445,14 +445,14 @@ class RolloutEngine:
         slots = torch.tensor(plan["seq_slots"], dtype=torch.int32).pin_memory().to(self.dev, non_blocking=True)
         tables = self.block_tables.index_select(0, slots.index_select(0, d[3 * n_rows:3 * n_rows + len(reqs)]))
         last: List[torch.Tensor] = []
-        for a, z, g0, g1, at, n_done in portions:
+        for a, z, g0, g1, at, n_done, pages in portions:
             k = g1 - g0
             starts, upto, done = d[at:at + k + 1], d[at + k + 1:at + 2 * k + 1], d[at + 2 * k + 1:at + 2 * k + 1 + n_done]
             x = torch.empty(z - a, cfg.hidden_size, dtype=torch.bfloat16, device=self.dev)
             C.embedding_fwd(d[a:z], dec.w("embed"), x)
             for i in range(cfg.num_hidden_layers):
                 x = dec.layer_fwd_paged(i, x, d[n_rows + a:n_rows + z], cos_t, sin_t, self._kc(i), self._vc(i), *self._scales(i),
-                                        d[2 * n_rows + a:2 * n_rows + z], tables[g0:g1], upto, starts)
+                                        d[2 * n_rows + a:2 * n_rows + z], tables[g0:g1, :pages], upto, starts)
             if n_done:
                 last.append(x.index_select(0, done))
         dec.launches += len(portions)

@@ -343,6 +343,38 @@ def test_a_page_that_does_not_exist_under_many_rows():
     assert int(c.status) == 0 and torch.equal(c.out, first)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("seqs", [[(1, 300)] * 3, [(40, 300), (300, 300)]])
+def test_output_rows_on_sixteen_bytes(seqs, eight):
+    c = Case(seqs, 12, 2, 128, 16, eight, pitch=8, seed=30)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_more_sequences_than_a_cta_has_at_hand(eight):
+    """Hundreds of idle sequences between those that have rows, in both kernels."""
+    for n in (1, 90):
+        seqs = [(n if b % 331 == 7 else 0, 100 + b % 9) for b in range(2000)]
+        c = Case(seqs, 12, 2, 128, 16, eight, seed=31)
+        c.call()
+        c.check()
+
+
+def test_tables_without_columns_and_rows_that_are_one_row():
+    c = Case([(4, 0), (2, 0)], 12, 2, 128, 16, False)
+    c.table = c.table[:, :0]
+    c.call()
+    assert bool((c.out == 0).all()) and int(c.status) == 0
+    c.lens[0] = 1  # more than its table holds
+    c.call()
+    assert int(c.status) == 6
+    one = Case([(300, 300)], 12, 2, 128, 16, True, seed=32)
+    one.rows = one.rows[:1].expand(300, -1)
+    one.call()
+    one.check()
+
+
 def test_pages_and_lengths_that_do_not_exist_are_reported():
     for page in (-1, 10 ** 6):
         c = Case([(1, 100), (1, 100)], 12, 2, 128, 16, False)
@@ -441,6 +473,9 @@ def test_refusals():
     small = torch.zeros(4, 2, 8, 128, dtype=torch.float8_e4m3fn, device=DEV)
     sc = torch.zeros(4, 2, 8, dtype=torch.uint8, device=DEV)
     refused("block size", k=small, v=small, ks=sc, vs=sc)
+    many = Case([(1, 1)] * 2048, 12, 2, 128, 16, True)  # of up to 2^29 tokens each
+    refused("too many rows", qkv=many.rows, lens=many.lens, starts=many.starts, out=many.out, k=many.kv[0], v=many.kv[1], ks=many.scales[0], vs=many.scales[1],
+            table=many.table[:1, :1].expand(2048, 1).new_zeros(1, 1 << 25).expand(2048, -1))
     # nothing to do
     native().paged_chunk_attn(c.rows[:0], c.kv[0], c.kv[1], c.table[:0], c.lens[:0], c.starts[:1], c.out[:0], 12, 2, 128, 0.1, c.status, c.scales[0], c.scales[1])
     assert bool((c.out == 7).all()) and int(c.status) == 0
