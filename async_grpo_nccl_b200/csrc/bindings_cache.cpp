@@ -13,6 +13,19 @@ namespace {
 
 using namespace cache_args;
 
+// Whether the first `cols` columns of `a` and those of `b`, as many rows of bf16, have nothing in common; both may be columns of one buffer.
+bool apart(const Tensor& a, const Tensor& b, int64_t cols) {
+  const int64_t n = a.size(0);
+  if (n == 0) return true;
+  const auto* x = static_cast<const c10::BFloat16*>(a.data_ptr());
+  const auto* y = static_cast<const c10::BFloat16*>(b.data_ptr());
+  if (y >= x + (n - 1) * a.stride(0) + cols || x >= y + (n - 1) * b.stride(0) + cols) return true;
+  const int64_t pitch = a.stride(0);
+  if (n == 1 || pitch <= 0 || b.stride(0) != pitch) return false;
+  const int64_t column = ((y - x) % pitch + pitch) % pitch;
+  return column >= cols && column + cols <= pitch;
+}
+
 void kv_cache_read(const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots, Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t D,
                    const OptTensor& status, const OptTensor& k_scale, const OptTensor& v_scale) {
   const char* op = "kv_cache_read";
@@ -39,7 +52,7 @@ void paged_chunk_attn(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_
   const torch::Device dev = qkv.device();
   written_rows(out, Hq * D, op, "out");
   TORCH_CHECK(out.device() == dev && out.size(0) == qkv.size(0) && out.size(1) == Hq * D, op, ": out [rows, Hq * D] on the device of the rows");
-  TORCH_CHECK(qkv.numel() == 0 || out.data_ptr() != qkv.data_ptr(), op, ": out must not be qkv");
+  TORCH_CHECK(apart(qkv, out, Hq * D), op, ": out must not be qkv or overlap its q heads");
   const agrpo::PagedCache c = cache(k_cache, v_cache, k_scale, v_scale, dev, D, op);
   TORCH_CHECK(c.Hkv == Hkv, op, ": cache of ", std::to_string(Hkv), " kv heads");
   TORCH_CHECK(c.block_size == 16 || c.block_size == 32 || c.block_size == 64 || c.block_size == 128, op, ": block size 16, 32, 64 or 128");

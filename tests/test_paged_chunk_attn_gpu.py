@@ -361,6 +361,17 @@ def test_more_sequences_than_a_cta_has_at_hand(eight):
         c.check()
 
 
+def test_rows_and_output_in_one_buffer():
+    for n in (1, 60):
+        c = Case([(n, 300)] * 3, 12, 2, 128, 16, False, seed=33)
+        both = torch.zeros(c.Tq, 2048 + 1536, dtype=torch.bfloat16, device=DEV)
+        for q, o in ((slice(0, 2048), slice(2048, 3584)), (slice(1536, 3584), slice(0, 1536))):
+            both[:, q] = c.rows
+            c.rows, c.out = both[:, q], both[:, o]
+            c.call()
+            c.check()
+
+
 def test_tables_without_columns_and_rows_that_are_one_row():
     c = Case([(4, 0), (2, 0)], 12, 2, 128, 16, False)
     c.table = c.table[:, :0]
@@ -465,6 +476,10 @@ def test_refusals():
     refused("out bf16", out=c.out.float())
     refused("must not be qkv", out=c.rows[:, :1536])
     refused("rows overlap", out=c.out[:1].expand(2, -1))
+    both = torch.zeros(2, 4096, dtype=torch.bfloat16, device=DEV)
+    refused("must not be qkv", qkv=both[:, :2048], out=both[:, 1528:3064])
+    refused("must not be qkv", qkv=both[:, 2048:], out=both[:, 1000:2536])
+    refused("must not be qkv", qkv=both[:, 8:2056], out=both[:, :1536])
     refused("q_starts int32", starts=c.starts.long())
     refused("seq_lens int32", lens=c.lens[:0])
     refused("block_tables", table=c.table.long())
