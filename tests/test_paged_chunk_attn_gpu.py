@@ -429,6 +429,30 @@ def test_a_cache_behind_two_gigabytes():
     assert torch.equal(c.out, first) and int(c.status) == 0
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_pages_behind_two_billion_elements(eight):
+    """A single token, some, and many (which an 8-bit cache is converted for)."""
+    Hkv, D, bs = 8, 128, 16
+    blocks = (1 << 31) // (Hkv * D * bs) + 400
+    for seqs in ([(1, 300), (1, 200)], [(9, 200), (40, 300)], [(1100, 1200)]):
+        c = Case(seqs, 16, Hkv, D, bs, eight, seed=34)
+        n = c.kv[0].shape[0]
+        big = [torch.empty(blocks, *k.shape[1:], dtype=torch.uint8 if eight else k.dtype, device=DEV) for k in c.kv]
+        scales = [torch.zeros(blocks, Hkv, bs, dtype=torch.uint8, device=DEV) if eight else None for _ in c.kv]
+        for b, k, s, t in zip(big, c.kv, scales, c.scales):
+            b[-n:] = k.view(torch.uint8) if eight else k
+            if eight:
+                s[-n:] = t
+        c.call()
+        first = c.out.clone()
+        c.kv = [b.view(torch.float8_e4m3fn) if eight else b for b in big]
+        c.scales = scales
+        c.table += blocks - n
+        c.out.fill_(7)
+        c.call()
+        assert torch.equal(c.out, first) and int(c.status) == 0
+
+
 def test_the_cache_that_was_written_is_what_is_attended():
     """Operators in a row, as an engine runs them: rows written in 8 bits, attended in place, and the same over what is read back."""
     C = native()
