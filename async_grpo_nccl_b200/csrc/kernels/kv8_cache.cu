@@ -127,9 +127,8 @@ __global__ void __launch_bounds__(kThreads) kv8_unpack_kernel(const __grid_const
     const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(is_v ? c.v : c.k) + src * D + lane * 16);
     const Kv8Scale s = kv8_scale((is_v ? c.v_scale : c.k_scale)[src]);
     const uint2 d = kv8_decode4(x.x, s), e = kv8_decode4(x.y, s), f = kv8_decode4(x.z, s), g = kv8_decode4(x.w, s);
-    uint4* y = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(is_v ? to.v : to.k) + dst * D + lane * 16);
-    y[0] = make_uint4(d.x, d.y, e.x, e.y);
-    y[1] = make_uint4(f.x, f.y, g.x, g.y);
+    const uint32_t y[8] = {d.x, d.y, e.x, e.y, f.x, f.y, g.x, g.y};
+    st_global_32b(static_cast<__nv_bfloat16*>(is_v ? to.v : to.k) + dst * D + lane * 16, y);
   }
 }
 
