@@ -1,6 +1,6 @@
 // KV cache in 8 bits: written from the rows of a prefill, written by a decode step with its rotation, read back into rows.
-// All three move bytes: a vector of D bf16 values is 2 D bytes on one side and D + 1 on the other. 16384 rows of 8 kv heads of 128 written and read back: 200 MB in
-// 46 us (4.4 TB/s), 21 and 20 us by themselves; what is left above the 31 us of memory is the address arithmetic, a third of the instructions.
+// All move bytes: a vector of D bf16 values is 2 D bytes on one side and D + 1 on the other. 16384 rows of 8 kv heads of 128 written and 16000 read back: 200 MB in
+// 41 - 45 us (4.4 - 4.9 TB/s), about as long each; what is left above the 31 us of memory is the address arithmetic, a third of the instructions.
 #include <cuda_bf16.h>
 
 #include "../common/ptx.cuh"
@@ -21,6 +21,29 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
+}
+
+// 16 bf16 values: a whole sector at once where they lie on one.
+__device__ __forceinline__ bool on_sector(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, uint4& a, uint4& b) {
+  if (on_sector(p)) {
+    uint32_t r[8];
+    ld_global_32b(p, r);
+    a = make_uint4(r[0], r[1], r[2], r[3]);
+    b = make_uint4(r[4], r[5], r[6], r[7]);
+  } else {
+    a = reinterpret_cast<const uint4*>(p)[0];
+    b = reinterpret_cast<const uint4*>(p)[1];
+  }
+}
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const uint4& a, const uint4& b) {
+  if (on_sector(p)) {
+    const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    st_global_32b(p, r);
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = a;
+    reinterpret_cast<uint4*>(p)[1] = b;
+  }
 }
 
 // Where vector `vec` of a call lies: row t, heads [0, Hkv) of K, then of V. 32-bit arithmetic: with 64-bit divisions the kernels were bound by them (16384 rows of 8 kv
@@ -62,9 +85,7 @@ kv8_write_kernel(const __nv_bfloat16* __restrict__ qkv, long long pitch, int k_c
   const Vector w = vector_at(min(vec, vectors - 1), c.Hkv);
   if (vec < vectors) at = place_of(c, slots[w.t], w.head, lane == 0, status);
   if (at >= 0) {
-    const auto* src = reinterpret_cast<const uint4*>(qkv + w.t * pitch + (w.is_v ? v_col0 : k_col0) + w.head * D + lane * 16);
-    x = src[0];
-    y = src[1];
+    load16(qkv + w.t * pitch + (w.is_v ? v_col0 : k_col0) + w.head * D + lane * 16, x, y);
   }
   const int byte = kv8_scale_byte(group_max<kLanes>(max(kv8_top(x), kv8_top(y))));
   if (at < 0) return;
@@ -85,19 +106,17 @@ kv_cache_read_kernel(PagedCache c, const int* __restrict__ slots, __nv_bfloat16*
   const Vector w = vector_at(vec, c.Hkv);
   const long long at = place_of(c, slots[w.t], w.head, lane == 0, status);
   if (at < 0) return;
-  uint4* dst = reinterpret_cast<uint4*>(qkv + w.t * pitch + (w.is_v ? v_col0 : k_col0) + w.head * D + lane * 16);
+  __nv_bfloat16* dst = qkv + w.t * pitch + (w.is_v ? v_col0 : k_col0) + w.head * D + lane * 16;
   const void* src = w.is_v ? c.v : c.k;
   if (k8) {
     const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + at * D + lane * 16);
     const Kv8Scale s = kv8_scale((w.is_v ? c.v_scale : c.k_scale)[at]);
     const uint2 a = kv8_decode4(x.x, s), b = kv8_decode4(x.y, s), d = kv8_decode4(x.z, s), e = kv8_decode4(x.w, s);
-    dst[0] = make_uint4(a.x, a.y, b.x, b.y);
-    dst[1] = make_uint4(d.x, d.y, e.x, e.y);
+    store16(dst, make_uint4(a.x, a.y, b.x, b.y), make_uint4(d.x, d.y, e.x, e.y));
   } else {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(src) + at * D + lane * 16);
-    const uint4 a = p[0], b = p[1];
-    dst[0] = a;
-    dst[1] = b;
+    uint4 a, b;
+    load16(static_cast<const __nv_bfloat16*>(src) + at * D + lane * 16, a, b);
+    store16(dst, a, b);
   }
 }
 

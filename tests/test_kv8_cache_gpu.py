@@ -144,6 +144,34 @@ def test_a_decode_step_rotates_and_writes(Hq, Hkv, D, B):
         assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("eight", [False, True])
+def test_rows_on_sixteen_bytes_read_and_write_the_same(D, eight):
+    """Every other row lies off the 32-byte sectors, a bf16 cache as a whole does."""
+    C = native()
+    T, Hq, Hkv, bs = 70, 3, 2, 16
+    cols = (Hq + 2 * Hkv) * D
+    x = rows_of(T, Hq + 2 * Hkv, D)
+    slots = torch.randperm(6 * bs, device=DEV)[:T].int()
+    seen = []
+    for pitch, off in ((0, 0), (8, 0), (8, 8)):
+        rows = torch.zeros(T, cols + pitch + off, device=DEV, dtype=torch.bfloat16)[:, off:off + cols]
+        rows.copy_(x)
+        scales = (None, None)
+        if eight:
+            k, v, *scales = empty_cache(6, Hkv, bs, D)
+        else:
+            k, v = (torch.zeros(6 * Hkv * bs * D + 8, device=DEV, dtype=torch.bfloat16)[off:off + 6 * Hkv * bs * D].view(6, Hkv, bs, D) for _ in range(2))
+        C.kv_cache_write(rows, slots, k, v, Hq, Hkv, D, None, 0, *scales)
+        back = torch.full((T, cols + pitch + off), 7.0, device=DEV, dtype=torch.bfloat16)[:, off:off + cols]
+        C.kv_cache_read(k, v, slots, back, Hq, Hkv, D, None, *scales)
+        assert bool((back[:, :Hq * D] == 7).all())
+        seen.append(back[:, Hq * D:].clone())
+    assert torch.equal(seen[1], seen[0]) and torch.equal(seen[2], seen[0])
+    if not eight:
+        assert torch.equal(seen[0], x[:, Hq * D:])
+
+
 def test_slots_behind_the_cache_are_reported_and_left_out():
     C = native()
     x = rows_of(3, 3, 64)
