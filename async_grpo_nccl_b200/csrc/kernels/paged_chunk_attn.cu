@@ -676,7 +676,7 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         break;
       }
       tc_fence_after();
-      if (any && busy && *odd != 0)
+      if (any && busy && __any_sync(0xffffffffu, *odd != 0))  // one answer for the warp
         l = add_taken_out<D, k8>(p, w.b, w.kvh, max(first_hidden(p, w.s, w.qb), w.j0 * kBN), min(unit_keys(p, w.s, w.qb), w.j1 * kBN), pos, tO, l);
       if (busy) {
         const bool whole = w.whole(), valid = r < rows;
