@@ -104,6 +104,7 @@ void bind_cache_ops(py::module_& m) {
         py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(), NOGIL,
         "Attention of the newest tokens of every sequence over the paged cache that already holds them. Sequence b owns the rows q_starts[b] .. "
         "q_starts[b + 1] of `qkv` (q heads in the first Hq D columns) and seq_lens[b] tokens of the cache; its row i of n sees the keys 0 .. "
-        "seq_lens[b] - n + i, a row that sees none is zero. Rows behind the last sequence are left as they are. Cache [blocks, Hkv, block size, D], "
+        "seq_lens[b] - n + i, a row that sees none is zero. Rows behind the last sequence are left as they are. Starts that go back "
+        "anywhere compute nothing, and the status word says so. Cache [blocks, Hkv, block size, D], "
         "bf16 or e4m3 with scale bytes. Nothing here reads the lengths on the host: a captured call follows them.");
 }

@@ -34,14 +34,15 @@ struct LineParams {
 
 struct Seq {
   int row0, n, len;
-  bool bad;
+  bool bad, back;  // does not fit its rows or its table; ends before it starts
 };
 __device__ __forceinline__ Seq load_seq(const LineParams& p, int b) {
   Seq s;
   s.row0 = p.a.q_starts[b];
   const int end = p.a.q_starts[b + 1];
   s.len = max(p.a.seq_lens[b], 0);
-  s.bad = s.row0 < 0 || end < s.row0 || end > p.a.Tq;
+  s.back = end < s.row0;
+  s.bad = s.row0 < 0 || s.back || end > p.a.Tq;
   s.n = s.bad ? 0 : end - s.row0;
   if (s.len > p.a.max_blocks * p.c.block_size) {
     s.bad = true;
@@ -64,7 +65,7 @@ struct SeqCache {
   __device__ __forceinline__ Seq get(const LineParams& p, int b) const {
     const int i = b - first;
     if (i >= room) return load_seq(p, b);
-    return Seq{at[3 * i], at[3 * i + 1], at[3 * i + 2], false};
+    return Seq{at[3 * i], at[3 * i + 1], at[3 * i + 2], false, false};
   }
 };
 // Keys that the last row of unit qb sees, and tiles of them. A unit without keys still has a tile: its rows are zeros to be written.
@@ -141,12 +142,14 @@ struct Walk {
 };
 
 // The line up to each sequence's end, into `line` (B ints of shared memory). All threads of the CTA; reports sequences that cannot be.
+// Starts that go back anywhere leave no line (its end, line[B - 1], is 0). Where they never do, no row belongs to two sequences, and the line is no longer
+// than paged_chunk_attn_tiles says; starts like 0, Tq, 0, Tq, .. would give all rows to every second sequence, and the sum could pass 31 bits.
 template <int kThreads, int kKeys, int kExtra>
 __device__ __forceinline__ void measure_line(const LineParams& p, int* line) {
   const int lane = threadIdx.x & 31;
   for (int base = 0; base < p.a.B; base += kThreads) {
     const int b = base + threadIdx.x;
-    Seq s = {0, 0, 0, false};
+    Seq s = {0, 0, 0, false, false};
     if (b < p.a.B) s = load_seq(p, b);
     if (s.bad && blockIdx.x == 0) report_status(p.a.status, kStatusBadIndex);
     const int units = num_units(p, s);
@@ -164,13 +167,15 @@ __device__ __forceinline__ void measure_line(const LineParams& p, int* line) {
       sum = __reduce_add_sync(0xffffffffu, sum);
       if (lane == src) mine = sum;
     }
-    if (b < p.a.B) line[b] = mine * p.c.Hkv;
+    if (b < p.a.B) line[b] = s.back ? -1 : mine * p.c.Hkv;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     int run = 0;
+    bool back = false;
     for (int base = 0; base < p.a.B; base += 32) {
       int v = base + lane < p.a.B ? line[base + lane] : 0;
+      back |= v < 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -180,6 +185,9 @@ __device__ __forceinline__ void measure_line(const LineParams& p, int* line) {
       run = __shfl_sync(0xffffffffu, v, 31);
       if (base + lane < p.a.B) line[base + lane] = v;
     }
+    back = __any_sync(0xffffffffu, back);
+    __syncwarp();
+    if (back && lane == 0) line[p.a.B - 1] = 0;
   }
   __syncthreads();
 }
@@ -236,7 +244,7 @@ __device__ __forceinline__ void locate(const LineParams& p, const int* line, int
 // A worker's share, of kLeast tiles at least if there are so many. One warp, all lanes with the same result.
 template <int kKeys, int kExtra, int kLeast>
 __device__ __forceinline__ Share find_share(const LineParams& p, const int* line, int worker, int workers) {
-  Share at = {0, 0, 0, 0, 0, 0, line[p.a.B - 1], 0, {0, 0, 0, false}};
+  Share at = {0, 0, 0, 0, 0, 0, line[p.a.B - 1], 0, {0, 0, 0, false, false}};
   at.workers = min(workers, (at.total + kLeast - 1) / kLeast);
   if (worker >= at.workers) return at;
   int end = share_start(at.total, worker + 1, at.workers);
