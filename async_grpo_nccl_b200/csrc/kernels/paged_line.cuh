@@ -279,7 +279,7 @@ __device__ __forceinline__ void add_parts(const float* part_ml, const float* par
     for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     const float Mn = fmaxf(M, mx);
     const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
-    const float wgt = ml.y != 0.f ? exp2f(ml.x - Mn) : 0.f;
+    const float wgt = ml.y != 0.f ? exp2f(ml.x - Mn) : -1.f;  // may be zero where there are keys: then 0 * NaN counts
     float ls = ml.y * wgt;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, off);
@@ -300,7 +300,7 @@ __device__ __forceinline__ void add_parts(const float* part_ml, const float* par
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float wi = __shfl_sync(0xffffffffu, wgt, i0 + i);
-        if (wi == 0.f) continue;  // no keys: what lies there means nothing
+        if (wi < 0.f) continue;  // no keys: what lies there means nothing
 #pragma unroll
         for (int d = 0; d < kPer; ++d) o[d] += x[i][d] * wi;
       }

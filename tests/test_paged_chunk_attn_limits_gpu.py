@@ -1,8 +1,9 @@
 """Attention of new tokens over the paged cache at the edge of what a call may hold."""
+import math
+
 import pytest
 import torch
 
-from gpu_util import native, status_word
 from test_paged_chunk_attn_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,31 @@ def test_starts_that_go_back_thousands_of_times(eight):
     c.call()
     assert int(c.status) == 6
     assert bool((c.out == 7).all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("kind", [math.nan, math.inf])
+@pytest.mark.parametrize("n,total", [(1, 3000), (3, 700), (1, 17), (40, 5000), (300, 600)])
+def test_values_that_are_no_numbers_count_under_any_probability(n, total, kind, eight):
+    """The first 64 tokens' logits lie so far below the others' (24 * 217 / 128^0.5 * log2 e: about 600 binades) that their probabilities are zero in 32 bits, in a
+    part of their own or not: 0 * NaN and 0 * inf are no numbers, whoever adds the parts."""
+    c = Case([(n, total)], 12, 2, 128, 16, eight, seed=n)
+    c.rows.copy_(c.rows.abs() + 0.5)  # |q| of 1.7 on average, 217 a head
+    for b in range(min(4, total // 16)):
+        page = int(c.table[0, b])
+        if eight:
+            c.kv[0].view(torch.uint8)[page] = 0xf4  # -192
+            c.scales[0][page] = 127 - 3                # times 2^-3
+        else:
+            c.kv[0][page] = -24
+    page = int(c.table[0, 0])
+    if eight:
+        c.scales[1][page, 1, 5] = 255
+    else:
+        c.kv[1][page, 1, 5, 7] = kind
+    c.call()
+    heads = c.out.view(n, 2, 6, 128)
+    assert bool(heads[:, 0].isfinite().all())
+    assert not bool(heads[:, 1, :, 7].isfinite().any())
+    if eight:
+        assert bool(heads[:, 1].isnan().all())
