@@ -484,7 +484,9 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
     }
     const bool whole = w.whole();
     const int part = w.part(warp) * F::kRows;
-    const float unit = k8 ? power(v_pow) : 1.f;
+    // The lift and F leave one after the other: values are then right from 2^-116 on (F over a sum of 2^13 and more would be below the smallest number) and up
+    // to a sum of 2^128, in parts as well.
+    const float unit = k8 ? power(v_pow) : 1.f, drop = k8 ? power(127 - static_cast<int>(kLift)) : 1.f;
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -496,27 +498,29 @@ __global__ void __launch_bounds__(Few<D, k8, kN>::kWarps * 32, 1) paged_few_attn
         if (r >= rows) continue;
         // a lane's dims: D / 8 from D / 8 * g on (8 bits), or 8 from 8 g (+ 64) on
         if (whole) {
-          const float f = sum != 0.f ? unit / sum : 0.f;
+          const float f = sum != 0.f ? 1.f / sum : 0.f;
+          const auto value = [&](float x) { return x * f * unit; };
           const int tk = r / G;
           auto* dst = static_cast<__nv_bfloat16*>(p.a.out) + (row0 + tk) * p.a.ldo + static_cast<long long>(w.kvh * G + r - tk * G) * D;
 #pragma unroll
           for (int i4 = 0; i4 < kSteps / 4; ++i4) {
             uint4 y;
-            y.x = pack_bf16x2(o[n][4 * i4][i] * f, o[n][4 * i4][i + 2] * f);
-            y.y = pack_bf16x2(o[n][4 * i4 + 1][i] * f, o[n][4 * i4 + 1][i + 2] * f);
-            y.z = pack_bf16x2(o[n][4 * i4 + 2][i] * f, o[n][4 * i4 + 2][i + 2] * f);
-            y.w = pack_bf16x2(o[n][4 * i4 + 3][i] * f, o[n][4 * i4 + 3][i + 2] * f);
+            y.x = pack_bf16x2(value(o[n][4 * i4][i]), value(o[n][4 * i4][i + 2]));
+            y.y = pack_bf16x2(value(o[n][4 * i4 + 1][i]), value(o[n][4 * i4 + 1][i + 2]));
+            y.z = pack_bf16x2(value(o[n][4 * i4 + 2][i]), value(o[n][4 * i4 + 2][i + 2]));
+            y.w = pack_bf16x2(value(o[n][4 * i4 + 3][i]), value(o[n][4 * i4 + 3][i + 2]));
             *reinterpret_cast<uint4*>(dst + (k8 ? D / 8 * g + 8 * i4 : 8 * g + 64 * i4)) = y;
           }
         } else {
           float* dst = part_o + (part + r) * D;
+          const auto value = [&](float x) { return x * drop * unit; };
 #pragma unroll
           for (int i2 = 0; i2 < kSteps / 2; ++i2) {
             const int dim = k8 ? D / 8 * g + 4 * i2 : 8 * g + 64 * (i2 / 2) + 4 * (i2 % 2);
             *reinterpret_cast<float4*>(dst + dim) =
-                make_float4(o[n][2 * i2][i] * unit, o[n][2 * i2][i + 2] * unit, o[n][2 * i2 + 1][i] * unit, o[n][2 * i2 + 1][i + 2] * unit);
+                make_float4(value(o[n][2 * i2][i]), value(o[n][2 * i2][i + 2]), value(o[n][2 * i2 + 1][i]), value(o[n][2 * i2 + 1][i + 2]));
           }
-          if (g == 0) *reinterpret_cast<float2*>(part_ml + (part + r) * 2) = make_float2(m[n][i], sum);
+          if (g == 0) *reinterpret_cast<float2*>(part_ml + (part + r) * 2) = make_float2(m[n][i], sum * drop);
         }
       }
     // A unit that starts in this warp and goes on, or that goes on from the CTA before: its parts in this CTA are added below.

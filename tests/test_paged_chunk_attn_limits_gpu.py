@@ -65,3 +65,20 @@ def test_values_that_are_no_numbers_count_under_any_probability(n, total, kind, 
     assert not bool(heads[:, 1, :, 7].isfinite().any())
     if eight:
         assert bool(heads[:, 1].isnan().all())
+
+
+@pytest.mark.parametrize("seqs,power", [([(1, 700)], 113), ([(1, 17)], 113), ([(2, 700)] * 40, 113), ([(40, 900)], 105), ([(1100, 1200)], 105),
+                                        ([(1, 700)], -110), ([(1, 17)], -110), ([(2, 700)] * 40, -110), ([(40, 900)], -110), ([(1100, 1200)], -110)])
+def test_eight_bit_values_near_the_ends_of_the_range(seqs, power):
+    """Values of 2^power. Sums are 32 bits, relative to a maximum that may be behind by 2 (few rows) or 8 binades: 700 * 2^2 * 2^(113 + 2.6) and 1200 * 2^8 * 2^(105 + 2.6)
+    are below 2^128. At the lower end a part of a row is off by 2^-126 for each key's product and each part, against 2^-8 * 2^-110 allowed."""
+    from async_grpo_nccl_b200.ops import reference as R
+
+    c = Case(seqs, 12, 2, 128, 16, True, seed=7)
+    held = c.scales[1] != 255
+    assert float(c.values[1].abs().max()) <= 2 ** 2.6
+    codes, s = R.kv8_quantise((c.values[1] * 2.0 ** power).bfloat16())
+    c.values[1] = R.kv8_values(codes, s)
+    c.kv[1], c.scales[1] = codes, s.masked_fill(~held, 255)
+    c.call()
+    c.check()
