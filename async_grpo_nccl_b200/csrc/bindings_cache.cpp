@@ -4,7 +4,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include <cmath>
+#include <limits>
 
 #include "bindings_layers.h"
 #include "launchers.h"
@@ -62,7 +62,9 @@ void paged_chunk_attn(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_
   TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.device() == dev && block_tables.dim() == 2 && block_tables.size(0) >= B &&
                   (block_tables.size(1) <= 1 || block_tables.stride(1) == 1), op, ": block_tables int32 [sequences, blocks], inner stride 1");
   TORCH_CHECK(B <= 8192 && block_tables.size(1) * c.block_size < (int64_t(1) << 30), op, ": at most 8192 sequences of 2^30 tokens");
-  TORCH_CHECK(std::isfinite(softmax_scale) && softmax_scale > 0, op, ": softmax_scale must be positive");
+  // in 32 bits, also times log2 e, and not a subnormal number: hidden scores are -inf, which times zero would be no number
+  TORCH_CHECK(softmax_scale >= std::numeric_limits<float>::min() && softmax_scale <= std::numeric_limits<float>::max() / 1.5, op,
+              ": softmax_scale must be a positive number of 32 bits");
   for (const OptTensor* s : {&k_scale, &v_scale}) TORCH_CHECK(!given(*s) || aligned16(**s), op, ": scales must be 16-byte aligned");
   status_word(status, dev, op);
   const c10::cuda::CUDAGuard guard(dev);

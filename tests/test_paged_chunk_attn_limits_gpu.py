@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+from async_grpo_nccl_b200.ops import reference as R
+from gpu_util import native
 from test_paged_chunk_attn_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -72,8 +74,6 @@ def test_values_that_are_no_numbers_count_under_any_probability(n, total, kind, 
 def test_eight_bit_values_near_the_ends_of_the_range(seqs, power):
     """Values of 2^power. Sums are 32 bits, relative to a maximum that may be behind by 2 (few rows) or 8 binades: 700 * 2^2 * 2^(113 + 2.6) and 1200 * 2^8 * 2^(105 + 2.6)
     are below 2^128. At the lower end a part of a row is off by 2^-126 for each key's product and each part, against 2^-8 * 2^-110 allowed."""
-    from async_grpo_nccl_b200.ops import reference as R
-
     c = Case(seqs, 12, 2, 128, 16, True, seed=7)
     held = c.scales[1] != 255
     assert float(c.values[1].abs().max()) <= 2 ** 2.6
@@ -82,3 +82,22 @@ def test_eight_bit_values_near_the_ends_of_the_range(seqs, power):
     c.kv[1], c.scales[1] = codes, s.masked_fill(~held, 255)
     c.call()
     c.check()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("n", [1, 60, 1100])
+def test_scales_that_32_bits_do_not_hold_are_refused(n, eight):
+    """A scale of zero in 32 bits would make hidden scores 0 * -inf. Next to that end it still is the mean of the values that a row sees."""
+    c = Case([(n, 1100)], 12, 2, 128, 16, eight, seed=3)
+
+    def call(scale):
+        native().paged_chunk_attn(c.rows, c.kv[0], c.kv[1], c.table, c.lens, c.starts, c.out, 12, 2, 128, scale, c.status, c.scales[0], c.scales[1])
+
+    for scale in (0.0, -0.1, math.nan, math.inf, 1e-60, 1e-39, 1e39, 3e38):
+        with pytest.raises(RuntimeError, match="softmax_scale"):
+            call(scale)
+    assert bool((c.out == 7).all())
+    call(1e-37)
+    want, size = R.paged_chunk_attention(c.rows, c.values[0], c.values[1], c.table, c.lens, c.starts, 12, 2, 128, 1e-37)
+    assert bool(((c.out.double() - want).abs() <= want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -10)).all())
+    assert int(c.status) == 0
