@@ -983,11 +983,19 @@ class RolloutEngine:
 
 
 # =====================================================================================================
+def refuse_cache_options(kv_cache_dtype: str, prefill_chunk_tokens: int) -> None:
+    """An engine without a cache gives bf16's results whatever these say, so it takes only their defaults."""
+    if kv_cache_dtype != "auto" or prefill_chunk_tokens != 0:
+        raise ValueError("kv_cache_dtype and prefill_chunk_tokens are options of the native rollout engine, which needs a GPU")
+
+
 class OracleEngine:
     """Same interface, plain PyTorch, full recompute per step. For tiny models on CPU and as a test oracle."""
 
     def __init__(self, cfg: ModelConfig, layout: ParamLayout, params: torch.Tensor, *, max_seqs: int = 64,
-                 max_model_len: Optional[int] = None, eos_token_id: Optional[int] = None, **_: Any):
+                 max_model_len: Optional[int] = None, eos_token_id: Optional[int] = None, kv_cache_dtype: str = "auto",
+                 prefill_chunk_tokens: int = 0, **_: Any):
+        refuse_cache_options(kv_cache_dtype, prefill_chunk_tokens)
         self.cfg, self.layout, self.params = cfg, layout, params
         self.dec = OracleDecoder(cfg, layout, params)
         self.max_model_len = int(max_model_len or cfg.max_position_embeddings)

@@ -147,6 +147,14 @@ def preflight_placement(place: Dict[str, Sequence[int]], world: int, visible_gpu
                              f"; each rank needs about {need_bytes / 2 ** 30:.1f} GiB (is another job using these GPUs?)")
 
 
+def _check_cache_options(config: GRPOConfig, native: bool) -> None:
+    """Options of the native rollout engine's cache, on every rank alike and ahead of any collective."""
+    if not native:
+        from .engine.engine import refuse_cache_options
+
+        refuse_cache_options(config.kv_cache_dtype, config.prefill_chunk_tokens)
+
+
 class InProcessRuntime:
     def __init__(self, config: GRPOConfig, device: Optional[str] = None, kv_memory_bytes: Optional[int] = None):
         self.config = config
@@ -154,6 +162,7 @@ class InProcessRuntime:
             config.param_sharding = "zero2"  # one trainer rank: nothing to shard over
         self.device = torch.device(device or ("cuda:0" if torch.cuda.is_available() else "cpu"))
         self.native = self.device.type == "cuda"
+        _check_cache_options(config, self.native)
         self.kv_memory_bytes = kv_memory_bytes
         self.trainer_ranks = [0]
         self.generation_controllers: List[Any] = []
@@ -438,6 +447,7 @@ class DistributedRuntime:
         self.config = config
         self.dist = dist
         cuda = torch.cuda.is_available()
+        _check_cache_options(config, cuda)
         if not dist.is_initialized():
             import datetime
 
