@@ -101,3 +101,19 @@ def test_scales_that_32_bits_do_not_hold_are_refused(n, eight):
     want, size = R.paged_chunk_attention(c.rows, c.values[0], c.values[1], c.table, c.lens, c.starts, 12, 2, 128, 1e-37)
     assert bool(((c.out.double() - want).abs() <= want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -10)).all())
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("seqs,Hq", [
+    ([(20 if b % 2 else 0, 100 + b % 9) for b in range(700)], 12),            # more sequences than the kernel has threads
+    ([(800 if b % 331 == 7 else 0, 800 + b % 9) for b in range(2000)], 12),   # hundreds of idle ones between those that have rows
+    ([(40 if b % 140 < 3 else 0, 60) for b in range(300)] * 2, 64),           # shares of short sequences go across idle ones
+    ([(900, 950)] * 3 + [(0, 40)] * 130 + [(900, 900)] * 3, 64),              # over 8 bits the cache is converted first
+    ([(1, 30 + b % 50) for b in range(3000)] + [(2500, 2500)], 64),           # single tokens beside a long prompt
+])
+def test_many_rows_among_many_sequences(seqs, Hq, eight):
+    """More sequences than a CTA has at hand (128) and than it has threads, in the kernel of many rows: Tq * (query heads a kv head) > 16 * sequences."""
+    assert sum(n for n, _ in seqs) * Hq // 2 > 16 * len(seqs)
+    c = Case(seqs, Hq, 2, 128, 16, eight, pad=1, seed=35)
+    c.call()
+    c.check()
