@@ -108,5 +108,8 @@ void bind_cache_ops(py::module_& m) {
         "q_starts[b + 1] of `qkv` (q heads in the first Hq D columns) and seq_lens[b] tokens of the cache; its row i of n sees the keys 0 .. "
         "seq_lens[b] - n + i, a row that sees none is zero. Rows behind the last sequence are left as they are. Starts that go back "
         "anywhere compute nothing, and the status word says so. Cache [blocks, Hkv, block size, D], "
-        "bf16 or e4m3 with scale bytes. Nothing here reads the lengths on the host: a captured call follows them.");
+        "bf16 or e4m3 with scale bytes. Nothing here reads the lengths on the host: a captured call follows them. For the same reason the kernel is "
+        "chosen by the average of rows over all sequences, and for 1024 rows (tokens times query heads of a kv head) a sequence over 8 bits the "
+        "cache is converted to bf16 in a workspace of up to 128 MB if full tables fit there: leave out sequences without rows, and pass tables as "
+        "wide as the longest sequence needs (a view will do).");
 }

@@ -1,6 +1,7 @@
 // KV cache in 8 bits: written from the rows of a prefill, written by a decode step with its rotation, read back into rows.
 // All move bytes: a vector of D bf16 values is 2 D bytes on one side and D + 1 on the other. 16384 rows of 8 kv heads of 128 written and 16000 read back: 200 MB in
-// 41 - 45 us (4.4 - 4.9 TB/s), about as long each; what is left above the 31 us of memory is the address arithmetic, a third of the instructions.
+// 41 - 45 us (4.4 - 4.9 TB/s), about as long each; what is left above the 31 us of memory is the address arithmetic, a third of the instructions,
+// and that a row is loaded when its slot is known (rows without a slot are not read). The bf16 cache read back: 16000 rows of 8 heads 22.8 us (5.7 TB/s).
 #include <cuda_bf16.h>
 
 #include "../common/ptx.cuh"

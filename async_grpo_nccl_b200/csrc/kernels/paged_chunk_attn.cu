@@ -352,7 +352,8 @@ paged_chunk_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         for (int t = 0; t < 2 && ok; ++t) {
           if (j >= end[t]) continue;
           if (j == w.j0 && n_o[t] > 0 && !wait(o_free + t, (n_o[t] - 1) & 1, kStatusWaitTmemEmptyTimeout)) break;
-          // The upper half's products run beside the lower half's exponentials (4096 tokens behind 12288: 694 -> 669 us). 8 bits: no gain, the warps that
+          // The upper half's products run beside the lower half's exponentials (4096 tokens behind 12288: 694 -> 669 us in a
+          // short loop; in one of seconds the power limit makes it 795). 8 bits: no gain, the warps that
           // convert are behind.
           using Half = std::integral_constant<int, kBN / 32>;
           if (!k8) {
@@ -764,7 +765,8 @@ void launch(LineParams p, int num_sms, void* scratch, cudaStream_t s) {
 }
 
 // Rows of a unit: 8 or 16 (the kernel of few rows) where the sequences have so many on average, else 256. (32 sequences of 2 to 6 rows of a group of 7 over 500
-// - 4000 tokens, bf16: 46 us here, 62 us in units of 16.)
+// - 4000 tokens, bf16: 46 us here, 62 us in units of 16.) The lengths are the device's, so the average counts sequences without rows: a few long prompts among hundreds of
+// idle ones take units of 8, single tokens beside one long prompt units of 256. The results are right, the time is not the best.
 int unit_rows(const ChunkAttnArgs& a, const PagedCache& c) {
   const int G = a.Hq / c.Hkv;
   const long long rows = static_cast<long long>(a.Tq) * G;
@@ -774,8 +776,8 @@ int unit_rows(const ChunkAttnArgs& a, const PagedCache& c) {
 
 // An 8-bit cache is converted to bf16 once, ahead of the attention, where every key would otherwise be converted for four units or more (on average): a tile of keys
 // takes a unit 1.4 times as long from 8 bits as from bf16, and writing it out as long as a third of such a tile. 4096 rows of 28 heads behind 12288 tokens
-// 955 -> 676 us; four units over 16000 tokens 51.4 -> 49.8, three 51.5 -> 54. Up to about the size of L2, where the copy stays; it is the allocator's again
-// after the call.
+// 955 -> 676 us (short loops); four units over 16000 tokens 51.4 -> 49.8, three 51.5 -> 54. Up to about the size of L2, where the copy stays; it is the allocator's again
+// after the call. The copy has room for full tables, whatever the lengths: tables wider than the longest sequence needs may be too wide for it.
 constexpr long long kUnpackMost = 128ll << 20;
 constexpr long long kUnpackRows = 1024;  // of a sequence
 struct Unpacked {
