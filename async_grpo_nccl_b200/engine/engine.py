@@ -75,6 +75,8 @@ class RolloutEngine:
         assert params.is_cuda
         self._check_model(cfg, params, block_size)
         self._init_cache_kind(kv_cache_dtype, int(prefill_chunk_tokens))
+        if (max_seqs if self.kv8 else min(max_seqs, self.prefill_chunk_tokens)) > 8192:
+            raise ValueError("the attention over the pages takes at most 8192 sequences: fewer max_seqs, or shorter portions over a bf16 cache")
         self.C = native()
         self.cfg, self.layout, self.params = cfg, layout, params
         self.dev = params.device

@@ -28,6 +28,14 @@ class Rounding:
             c[at // c.shape[2], :, at % c.shape[2]] = R.kv8_values(*R.kv8_quantise(rows)).to(torch.bfloat16)
 
 
+@pytest.mark.parametrize("kw", [dict(kv_cache_dtype="fp8"), dict(prefill_chunk_tokens=8193)])
+def test_more_sequences_than_the_attention_takes_are_refused_at_once(model, kw):  # noqa: F811
+    with pytest.raises(ValueError, match="8192"):
+        engine(model, max_seqs=8193, **kw)
+    if "prefill_chunk_tokens" in kw:
+        engine(model, max_seqs=8193, prefill_chunk_tokens=64)
+
+
 @pytest.mark.parametrize("size", [100, 100000])
 def test_prompts_over_8_bits_are_prompts_over_rounded_keys_and_values(model, size):  # noqa: F811
     prompts = prompts_of(model[0], [90, 130, 260, 400])
